@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "params.h"
+#include "w8a8.h"
 
 namespace glowq {
 size_t gemv_smem_bytes(const GemvParams& p, int NT);
@@ -209,6 +210,28 @@ int tensor_map_w3d(CUtensorMap* out, const void* ptr, uint64_t group_pairs, uint
   std::memcpy(out, &slot.map, sizeof(CUtensorMap));
   return GLOWQ_OK;
 }
+
+}  // namespace
+
+// Shared with the 8-bit path.
+namespace glowq {
+int current_device_sms(int* sms) {
+  const DeviceInfo* dev = nullptr;
+  const int rc = device_info(&dev);
+  if (rc == GLOWQ_OK) *sms = dev->sms;
+  return rc;
+}
+int note_cuda_error(cudaError_t e) { return e == cudaSuccess ? GLOWQ_OK : fail_cuda(e); }
+bool use_pdl() {
+  static const bool on = [] {
+    const char* v = std::getenv("GLOWQ_PDL");
+    return !(v && v[0] == '0');
+  }();
+  return on;
+}
+}  // namespace glowq
+
+namespace {
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }

@@ -1,0 +1,39 @@
+// Launch functions of the 8-bit path, shared by its translation units.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/glowq_w8a8.h"
+
+namespace glowq {
+
+// abi.cu
+int tensor_map_2d_ex(CUtensorMap* out, CUtensorMapDataType dtype, const void* ptr, uint64_t dim0, uint64_t dim1,
+                     uint64_t stride_bytes, uint32_t box0, uint32_t box1, int swizzle);
+int current_device_sms(int* sms);          // GLOWQ_* status: the current device is one that the library runs on
+int note_cuda_error(cudaError_t e);        // GLOWQ_OK, or GLOWQ_ERR_CUDA with the error kept for glowq_w4a16_last_cuda_error
+bool use_pdl();
+
+// w8a8_rows.cu
+cudaError_t launch_rows(const glowq_w8a8_rows_t& p, cudaStream_t stream);
+cudaError_t launch_layer_norm_grad(const glowq_layer_norm_grad_t& g, cudaStream_t stream);
+size_t layer_norm_grad_bytes(int M, int K);
+
+// w8a8_stream.cu
+int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stream);
+int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool early, int sms, cudaStream_t stream);
+cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream);
+
+// Reads a file's status word and clears it.
+template <typename Symbol> cudaError_t take_status(Symbol& word, uint32_t* out, cudaStream_t stream) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(out, word, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess || *out == 0) return e;
+  static const uint32_t zero = 0;
+  return cudaMemcpyToSymbolAsync(word, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream);
+}
+
+inline size_t dtype_bytes(int dtype) { return dtype == GLOWQ_F32 ? 4 : 2; }
+
+}  // namespace glowq

@@ -1,0 +1,279 @@
+"""Token codes and the 8-bit linear as functions of tensors.
+
+    scale_t = fp32(max_k |x_tk| / 127)        code_tk = the integer nearest to x_tk / scale_t, ties to even, of the exact quotient
+    y_to    = scale_t * weight_scale_o * sum_k code_tk weight_ok  +  alpha * sum_j r_tj L_oj  (+ bias_o),      r = x R^T
+
+The sums of products are exact; the rest is fp32, rounded once to the output's type.  A token with a NaN or an infinity has scale NaN and
+all its outputs are NaN; other tokens do not see it.  Everything runs on the current stream of the tensors' device, allocates its outputs
+and its scratch through PyTorch, and works under a captured graph.  There are no gradients here (as in ``CudaW4A16Linear``); the layer
+norm has them (``layer_norm``)."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from ..cuda_w4a16.kernels import current_stream_ptr
+from . import kernels as K
+
+_NORMS = {"layer": K.NORM_LAYER, "rms": K.NORM_RMS}
+_pack_rows, _pack_linear = K.pack_rows.pack, K.pack_linear.pack
+
+
+class TokenCodes(NamedTuple):
+    """A linear's input as int8 codes [tokens, in_features] with an fp32 scale per token [tokens].  ``r``: the right factor's product
+    with the same input, fp16 [tokens, rank], for corrected linears that share one.  Rows of codes lie a multiple of 16 bytes apart."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    r: Optional[torch.Tensor] = None
+
+
+def _pitch(k: int) -> int:
+    return (k + 15) & ~15
+
+
+def _new_codes(m: int, k: int, device) -> torch.Tensor:
+    pitch = _pitch(k)
+    t = torch.empty((m, pitch), dtype=torch.int8, device=device)
+    return t if pitch == k else t[:, :k]
+
+
+def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    """``x`` as [rows, columns] with unit column stride and rows that do not overlap."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be CUDA (sm_100); there is no CPU path")
+    if x.dtype not in K.DTYPES:
+        raise RuntimeError(f"{name} must be fp16, bf16 or fp32, got {x.dtype}")
+    if x.dim() != 2:
+        if x.dim() == 0:
+            raise RuntimeError(f"{name} must have a last dimension")
+        x = x.reshape(-1, x.shape[-1])
+    if x.shape[1] == 0:
+        raise RuntimeError(f"{name} must have columns")
+    stride = x.stride()
+    if (stride[1] != 1 and x.shape[1] > 1) or (stride[0] < x.shape[1] and x.shape[0] > 1):
+        x = x.contiguous()
+    return x
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the copy engine reads it: rows that begin on 16 bytes.  (Others are copied; what the package makes lies so.)"""
+    e = t.element_size()
+    stride = t.stride()
+    if t.data_ptr() % 16 == 0 and (stride[1] == 1 or t.shape[1] == 1) and (
+            t.shape[0] <= 1 or (stride[0] * e % 16 == 0 and stride[0] >= t.shape[1])):
+        return t
+    cols = 16 // e
+    room = torch.empty((t.shape[0], (t.shape[1] + cols - 1) // cols * cols), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+    room.copy_(t)
+    return room
+
+
+def _operand_stride(t: torch.Tensor) -> int:
+    """(of a single row the stride may be anything; the library is told one that it accepts)"""
+    cols = 16 // t.element_size()
+    return t.stride()[0] if t.shape[0] > 1 else (t.shape[1] + cols - 1) // cols * cols
+
+
+def _quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, constant: bool) -> None:
+    desc = _pack_rows(x.data_ptr(), 0, 0, 0, 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0, current_stream_ptr(x.device), 0.0,
+                      x.stride()[0], 0, 0, 0, codes.stride()[0], x.shape[0], x.shape[1], K.DTYPES[x.dtype], K.NORM_NONE, constant, 0)
+    K.call(K.ext().quantize, x.device, desc, "glowq_w8a8_quantize")
+
+
+def quantize_tokens(x: torch.Tensor) -> TokenCodes:
+    """int8 codes and a scale for every row of ``x`` [..., in_features] (fp16, bf16 or fp32), in one launch."""
+    x = _rows(x.detach(), "x")
+    m, k = x.shape
+    codes = _new_codes(m, k, x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    if m:
+        _quantize(x, codes, scales, False)
+    return TokenCodes(codes, scales)
+
+
+def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of a weight [out_features, in_features], a scale for every output channel.  The codes are a view of rows that lie a
+    multiple of 16 bytes apart.  On the CPU the same codes with torch expressions, so that a model can be converted there."""
+    if weight.dim() != 2 or weight.dtype not in K.DTYPES:
+        raise RuntimeError("weight must be [out_features, in_features] in fp16, bf16 or fp32")
+    weight = weight.detach()
+    oc, ic = weight.shape
+    codes = torch.zeros((oc, _pitch(ic)), dtype=torch.int8, device=weight.device)[:, :ic]
+    scales = torch.empty(oc, dtype=torch.float32, device=weight.device)
+    if oc == 0:
+        return codes, scales
+    if weight.is_cuda:
+        _quantize(_rows(weight, "weight"), codes, scales, True)
+        return codes, scales
+    top = weight.float().abs().amax(dim=1)
+    torch.div(top, torch.full_like(top, 127.0), out=scales)
+    bad = ~torch.isfinite(top)
+    scales[bad] = float("nan")
+    q = torch.round(weight.double() / scales.double()[:, None]).clamp_(-127, 127)
+    codes.copy_(torch.where((scales > 0)[:, None], q, torch.zeros_like(q)))
+    return codes, scales
+
+
+def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                         residual: Optional[torch.Tensor] = None, norm: str = "rms") -> Tuple[TokenCodes, torch.Tensor]:
+    """Residual add, norm and codes in one launch: (codes of norm(h), h) with h = x + residual (h is ``x`` itself without a residual).
+
+    ``norm``: "layer" (``nn.LayerNorm``'s arithmetic, ``bias`` may be None) or "rms" (the models' RMSNorm modules: fp32 statistics, the
+    normalised value rounded to the input's type before the weight).  All tensors have one type; h and the normalised values are
+    rounded to it, so the codes are those of the separate steps."""
+    kind = _NORMS.get(norm)
+    if kind is None:
+        raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
+    if kind == K.NORM_RMS and bias is not None:
+        raise ValueError("RMSNorm has no bias")
+    x2 = _rows(x.detach(), "x")
+    m, k = x2.shape
+    check_norm(x2, weight, bias, eps)
+    res, hidden = residual, x
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise RuntimeError("residual must have x's shape, type and device")
+        res = _rows(residual.detach(), "residual")
+        hidden = torch.empty((m, k), dtype=x.dtype, device=x.device)
+    codes = _new_codes(m, k, x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    if m:
+        w = weight.detach().contiguous()
+        b = bias.detach().contiguous() if bias is not None else None
+        with_res = res is not None
+        desc = _pack_rows(x2.data_ptr(), res.data_ptr() if with_res else 0, w.data_ptr(), b.data_ptr() if b is not None else 0,
+                          hidden.data_ptr() if with_res else 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0,
+                          current_stream_ptr(x.device), float(eps), x2.stride()[0], res.stride()[0] if with_res else 0, k, 0,
+                          codes.stride()[0], m, k, K.DTYPES[x.dtype], kind, 0, 0)
+        K.call(K.ext().quantize, x.device, desc, "glowq_w8a8_quantize")
+    if residual is not None:
+        hidden = hidden.reshape(x.shape)
+    return TokenCodes(codes, scales), hidden
+
+
+def check_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
+    """(``x``: what ``_rows`` gave)"""
+    k = x.shape[1]
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None and name == "bias":
+            continue
+        if t is None or t.dim() != 1 or t.shape[0] != k or t.dtype != x.dtype or t.device != x.device:
+            raise RuntimeError(f"{name} must be [{k}] of x's type on x's device")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+
+
+def _factor(t: torch.Tensor, name: str, rows: int, cols: Optional[int], device) -> torch.Tensor:
+    if t.dim() != 2 or t.dtype != torch.float16 or t.device != device or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
+        raise RuntimeError(f"{name} must be fp16 [{rows}, {'rank' if cols is None else cols}] on {device}, got {t.dtype} {tuple(t.shape)}")
+    return _operand(t.detach())
+
+
+def right_factor(x: torch.Tensor, R: torch.Tensor) -> torch.Tensor:
+    """r = x R^T, fp16 [tokens, rank], for corrected linears that share a right factor (``TokenCodes.r``).  ``x`` is taken in fp16, as the
+    W4A16 path takes it; sums in fp32."""
+    x = _rows(x.detach(), "x")
+    if R.dim() != 2 or not 0 < R.shape[0] <= K.MAX_RANK:
+        raise RuntimeError(f"R must be [rank, in_features] with a rank of 1 to {K.MAX_RANK}")
+    m, k = x.shape
+    R = _factor(R, "R", R.shape[0], k, x.device)
+    rank = R.shape[0]
+    r = torch.empty((m, (rank + 7) & ~7), dtype=torch.float16, device=x.device)[:, :rank]
+    if m:
+        x = _operand(x if x.dtype == torch.float16 else x.to(torch.float16))
+        desc = _pack_linear(0, 0, 0, 0, 0, 0, x.data_ptr(), R.data_ptr(), r.data_ptr(), 0, 0, current_stream_ptr(x.device), 0, 0, 0,
+                            _operand_stride(x), _operand_stride(R), _operand_stride(r), 0, 0, m, k, 0, rank, 0, 0, K.R_COMPUTE, 0.0, 0)
+        K.call(K.ext().right_factor, x.device, desc, "glowq_w8a8_right_factor")
+    return r
+
+
+def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight_scales: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, *, out_dtype: Optional[torch.dtype] = None, L: Optional[torch.Tensor] = None,
+                R: Optional[torch.Tensor] = None, alpha: float = 1.0) -> torch.Tensor:
+    """One 8-bit linear.  ``x``: activations [..., in_features] (their codes are made here), or ``TokenCodes`` -> [tokens, out_features].
+    ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
+    [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, fp16 for codes.  ``L`` fp16 [out_features, rank]:
+    the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``."""
+    if isinstance(x, TokenCodes):
+        codes, scales, r = x.codes, x.scales, x.r
+        if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2:
+            raise RuntimeError("codes must be int8 [tokens, in_features] on a CUDA device")
+        m, k = codes.shape
+        dev = codes.device
+        if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != m or scales.device != dev:
+            raise RuntimeError(f"scales must be fp32 [{m}] on {dev}")
+        codes, scales = _operand(codes), scales.contiguous()
+        x2, lead = None, None
+        if R is not None:
+            raise RuntimeError("codes have no right factor's product to be made from: pass TokenCodes.r (right_factor(x, R))")
+        if out_dtype is None:
+            out_dtype = torch.float16
+    else:
+        x2, r = _rows(x.detach(), "x"), None
+        m, k = x2.shape
+        dev, lead = x2.device, x.shape
+        if (L is None) != (R is None):
+            raise RuntimeError("a correction needs L and R")
+        if out_dtype is None:
+            out_dtype = x2.dtype
+    out_code = K.DTYPES.get(out_dtype)
+    if out_code is None:
+        raise RuntimeError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
+    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.device != dev:
+        raise RuntimeError(f"weight must be int8 [out_features, in_features] on {dev}")
+    if weight.shape[1] != k:
+        raise ValueError(f"Input dim mismatch: got {k}, expected {weight.shape[1]}")
+    if not 0 < k <= K.MAX_EXACT_K:
+        raise RuntimeError(f"in_features must be 1 to {K.MAX_EXACT_K} (sums are exact in 32 bits)")
+    oc = weight.shape[0]
+    for t, name in ((weight_scales, "weight_scales"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != oc or t.device != dev):
+            raise RuntimeError(f"{name} must be fp32 [{oc}] on {dev}")
+    if m > K.MAX_TOKENS:
+        raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
+    out = torch.empty((m, oc), dtype=out_dtype, device=dev)
+    if m and oc:
+        weight, weight_scales = _operand(weight), weight_scales.contiguous()
+        bias = bias.detach().contiguous() if bias is not None else None
+        rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = 0
+        if L is not None:
+            L = _factor(L, "L", oc, None, dev)
+            rank = L.shape[1]
+            if not 0 < rank <= K.MAX_RANK:
+                raise RuntimeError(f"the rank must be 1 to {K.MAX_RANK}")
+            L_at, L_stride = L.data_ptr(), _operand_stride(L)
+            if x2 is None:
+                if r is None:
+                    raise RuntimeError("a corrected linear of codes needs TokenCodes.r (right_factor(x, R))")
+                r = _factor(r, "r", m, rank, dev)
+                mode, r_at, r_stride = K.R_LOAD, r.data_ptr(), _operand_stride(r)
+            else:
+                R = _factor(R, "R", rank, k, dev)
+                rx = _operand(x2 if x2.dtype == torch.float16 else x2.to(torch.float16))
+                mode, R_at, R_stride, rx_at, rx_stride = K.R_COMPUTE, R.data_ptr(), _operand_stride(R), rx.data_ptr(), _operand_stride(rx)
+        x_at = x_stride = x_code = 0
+        if x2 is None:
+            code_at, code_stride, scale_at = codes.data_ptr(), _operand_stride(codes), scales.data_ptr()
+        else:
+            # codes, scales and r of this call: one piece of memory
+            x_at, x_stride, x_code = x2.data_ptr(), x2.stride()[0], K.DTYPES[x2.dtype]
+            code_stride, r_stride = _pitch(k), (rank + 7) & ~7
+            scale_off = m * code_stride
+            r_off = scale_off + (4 * m + 15 & ~15)
+            room = torch.empty(r_off + 2 * m * r_stride, dtype=torch.uint8, device=dev)
+            code_at = room.data_ptr()
+            scale_at, r_at = code_at + scale_off, code_at + r_off
+        desc = _pack_linear(x_at, code_at, scale_at, weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr() if bias is not None else 0,
+                            rx_at, R_at, r_at, L_at, out.data_ptr(), current_stream_ptr(dev), x_stride, code_stride,
+                            _operand_stride(weight), rx_stride, R_stride, r_stride, L_stride, oc, m, k, oc, rank, x_code, out_code, mode,
+                            float(alpha), 0)
+        K.call(K.ext().linear, dev, desc, "glowq_w8a8_linear")
+    return out if lead is None or len(lead) == 2 else out.reshape(*lead[:-1], oc)
+
+
+def read_status(device: Optional[torch.device] = None) -> None:
+    """Raises if a bounded wait of the 8-bit kernels has run out on the device since the last call.  Synchronises the current stream."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(device):
+        K.ext().check(K.ext().lib.glowq_w8a8_read_status(torch.cuda.current_stream().cuda_stream), "device status")
