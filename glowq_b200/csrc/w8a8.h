@@ -25,6 +25,10 @@ int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stre
 int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool early, int sms, cudaStream_t stream);
 cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream);
 
+// w8a8_pair.cu: tiles of 256 tokens x n channels (64, 128, 192 or 256)
+int w8a8_pair_forward(const glowq_w8a8_linear_t& g, int n, int sms, cudaStream_t stream);
+cudaError_t w8a8_pair_status(uint32_t* out, cudaStream_t stream);
+
 // Reads a file's status word and clears it.
 template <typename Symbol> cudaError_t take_status(Symbol& word, uint32_t* out, cudaStream_t stream) {
   cudaError_t e = cudaMemcpyFromSymbolAsync(out, word, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, stream);

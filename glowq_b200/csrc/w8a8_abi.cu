@@ -1,4 +1,7 @@
 // Entry points declared in include/glowq_w8a8.h: checks of the arguments and dispatch.
+#include <cmath>
+#include <cstdlib>
+
 #include "w8a8.h"
 
 using namespace glowq;
@@ -80,6 +83,25 @@ int check_linear(const glowq_w8a8_linear_t& g) {
   return rc;
 }
 
+// Channels of a pair's tile, or 0: the streaming form.
+int pair_columns(const glowq_w8a8_linear_t& g, int sms) {
+  if (const char* v = std::getenv("W8_TILE")) return std::atoi(v);
+  if (g.M <= 128) return 0;
+  // (a converted tile is held as sums / alpha: a factor near nothing would leave the range of fp32)
+  if (g.r_mode != GLOWQ_R_NONE && !(std::fabs(g.alpha) >= 0x1p-60f && std::fabs(g.alpha) <= 0x1p60f)) return 0;
+  const int n_y = (g.M + 255) / 256, pairs = sms / 2;
+  int best = 256;
+  long long best_cost = 0;
+  for (int n = 256; n >= 64; n -= 64) {
+    const long long tiles = static_cast<long long>((g.OC + n - 1) / n) * n_y, cost = (tiles + pairs - 1) / pairs * (2 * n + 60);
+    if (n == 256 || cost < best_cost) {
+      best = n;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 extern "C" {
@@ -119,11 +141,12 @@ int glowq_w8a8_right_factor(const glowq_w8a8_linear_t* linear) {
 
 int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
   if (!linear) return GLOWQ_ERR_BAD_ARGUMENT;
-  const glowq_w8a8_linear_t& g = *linear;
+  glowq_w8a8_linear_t g = *linear;
   int rc = check_linear(g), sms = 0;
   if (rc == GLOWQ_OK) rc = current_device_sms(&sms);
   if (rc != GLOWQ_OK || g.M == 0) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(g.stream);
+  if (g.alpha == 0.f) g.r_mode = GLOWQ_R_NONE;   // nothing to add
   if (g.x) {
     glowq_w8a8_rows_t r{};
     r.x = g.x;
@@ -137,13 +160,15 @@ int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
     if ((rc = note_cuda_error(launch_rows(r, stream))) != GLOWQ_OK) return rc;
   }
   if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, true, sms, stream)) != GLOWQ_OK) return rc;
-  return w8a8_stream_forward(g, sms, stream);
+  const int n = pair_columns(g, sms);
+  return n > 0 ? w8a8_pair_forward(g, n, sms, stream) : w8a8_stream_forward(g, sms, stream);
 }
 
 int glowq_w8a8_read_status(void* stream) {
-  uint32_t word = 0;
-  const int rc = note_cuda_error(w8a8_stream_status(&word, static_cast<cudaStream_t>(stream)));
-  return rc != GLOWQ_OK ? rc : word ? GLOWQ_ERR_DEVICE_TIMEOUT : GLOWQ_OK;
+  uint32_t words[2] = {0, 0};
+  int rc = note_cuda_error(w8a8_stream_status(&words[0], static_cast<cudaStream_t>(stream)));
+  if (rc == GLOWQ_OK) rc = note_cuda_error(w8a8_pair_status(&words[1], static_cast<cudaStream_t>(stream)));
+  return rc != GLOWQ_OK ? rc : words[0] | words[1] ? GLOWQ_ERR_DEVICE_TIMEOUT : GLOWQ_OK;
 }
 
 }  // extern "C"

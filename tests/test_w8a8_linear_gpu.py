@@ -8,6 +8,12 @@ from w8a8_reference import HALF_STEP, U, assert_within, codes_of, product_of
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    w8.read_status()
+
+
 def operands(m, k, n, rank=0, bias=True, seed=0, dtype=torch.float16):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731

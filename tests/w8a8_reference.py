@@ -43,6 +43,10 @@ def product_of(codes, scales, weight, weight_scales, bias, alpha=0.0, r=None, L=
         y += alpha * (r.double() @ L.double().t())
         mag = abs(alpha) * (r.double().abs() @ L.double().abs().t())
         bound += (2 * r.shape[1] + 4) * U * mag  # sums of rank products whose adder may truncate: two half steps each
+        # the products may be added to the scaled sum itself, held as sum / alpha (three more roundings: 1 / alpha, the quotient, the
+        # product with alpha), by four MMAs for every 64 ranks, each of which may truncate the sum
+        rest = p.abs() + (bias.double().abs() if bias is not None else 0)
+        bound += (3 + 8 * ((r.shape[1] + 63) // 64)) * U * rest
     if bias is not None:
         y += bias.double()
         bound += 2 * U * bias.double().abs()
