@@ -16,7 +16,7 @@ int note_cuda_error(cudaError_t e);        // GLOWQ_OK, or GLOWQ_ERR_CUDA with t
 bool use_pdl();
 
 // w8a8_rows.cu
-cudaError_t launch_rows(const glowq_w8a8_rows_t& p, cudaStream_t stream);
+cudaError_t launch_rows(const glowq_w8a8_rows_t& p, int sms, cudaStream_t stream);
 cudaError_t launch_layer_norm_grad(const glowq_layer_norm_grad_t& g, cudaStream_t stream);
 size_t layer_norm_grad_bytes(int M, int K);
 

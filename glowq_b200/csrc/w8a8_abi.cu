@@ -41,7 +41,7 @@ int run_rows(const glowq_w8a8_rows_t* rows, bool codes) {
   int rc = check_rows(*rows, codes), sms = 0;
   if (rc == GLOWQ_OK) rc = current_device_sms(&sms);
   if (rc != GLOWQ_OK || rows->M == 0) return rc;
-  return note_cuda_error(launch_rows(*rows, static_cast<cudaStream_t>(rows->stream)));
+  return note_cuda_error(launch_rows(*rows, sms, static_cast<cudaStream_t>(rows->stream)));
 }
 
 // operands that the copy engine reads: they begin on 16 bytes, and so does every row
@@ -157,7 +157,7 @@ int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
     r.M = g.M;
     r.K = g.K;
     r.dtype = g.x_dtype;
-    if ((rc = note_cuda_error(launch_rows(r, stream))) != GLOWQ_OK) return rc;
+    if ((rc = note_cuda_error(launch_rows(r, sms, stream))) != GLOWQ_OK) return rc;
   }
   if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, true, sms, stream)) != GLOWQ_OK) return rc;
   const int n = pair_columns(g, sms);
