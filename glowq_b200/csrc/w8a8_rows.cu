@@ -283,6 +283,40 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void store_row(T* r
   }
 }
 
+// ---------------------------------------------------------------- two fp32 values in one instruction
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair_of(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <typename T> __device__ __forceinline__ void unpack2(const Vec& v, F2 (&f)[Num<T>::kVec / 2]) {
+  float u[Num<T>::kVec];
+  Num<T>::unpack(v, u);
+#pragma unroll
+  for (int i = 0; i < Num<T>::kVec / 2; ++i) f[i] = pair_of(u[2 * i], u[2 * i + 1]);
+}
+
 // ---------------------------------------------------------------- codes
 struct Scale {
   float s, lo, hi;   // the scale; a little less and a little more than its inverse
@@ -662,7 +696,7 @@ template <typename T> cudaError_t launch_rows_typed(const RowsParams& p, int nor
 // rows at a time, and the next ones' loads go out before these are worked on.  A thread keeps to its columns: the sums of dweight and
 // dbias stay in its registers until the end.  Reads h, dy (dh) and writes dx once: bound by memory.
 constexpr int kGradParts = 296;    // CTAs of the gradients at most, whatever the device: their number fixes the order of the sums
-constexpr int kGradThreads = 512;
+constexpr int kGradThreads = 1024;
 
 struct GradParams {
   const void *h, *dy, *dh, *weight;
@@ -681,12 +715,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
   const int g = threadIdx.x / p.group, t = threadIdx.x - g * p.group, groups = blockDim.x / p.group, step = p.group * V, K = p.K;
   const int nw = p.group >> 5, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  float w[NV][V], dw[NV][V], db[NV][V];
+  F2 w[NV][V / 2], dw[NV][V / 2], db[NV][V / 2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    Num<T>::unpack(load_row<T, WHOLE>(static_cast<const T*>(p.weight), t * V + i * step, K), w[i]);
+    unpack2<T>(load_row<T, WHOLE>(static_cast<const T*>(p.weight), t * V + i * step, K), w[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+    for (int j = 0; j < V / 2; ++j) dw[i][j] = db[i][j] = 0ull;
   }
   const float inv_k = 1.f / static_cast<float>(K);
   Vec nh[ROWS][NV], nd[ROWS][NV];
@@ -712,70 +746,86 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
   for (int base = blockIdx.x * groups * ROWS; base < p.M; base += stride, buf ^= 1) {   // (the same number of rounds for all groups)
     const int r0 = base + g * ROWS;
     // xh = h rstd - mean rstd, and dy; zeros past the end of a row (dy) and past the last row (dy)
-    float xh[ROWS][NV][V], d[ROWS][NV][V], rstd[ROWS];
+    F2 xh[ROWS][NV][V / 2], d[ROWS][NV][V / 2];
+    float rstd[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       rstd[r] = nrstd[r];
-      const float shift = -nmean[r] * rstd[r];
+      const F2 rs2 = pair_of(rstd[r], rstd[r]), shift = pair_of(-nmean[r] * rstd[r], -nmean[r] * rstd[r]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        Num<T>::unpack(nh[r][i], xh[r][i]);
-        Num<T>::unpack(nd[r][i], d[r][i]);
+        unpack2<T>(nh[r][i], xh[r][i]);
+        unpack2<T>(nd[r][i], d[r][i]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) xh[r][i][j] = fmaf(xh[r][i][j], rstd[r], shift);
+        for (int j = 0; j < V / 2; ++j) xh[r][i][j] = fma2(xh[r][i][j], rs2, shift);
       }
     }
     if (base + stride < p.M) fetch(r0 + stride);
     // sums of dy w and dy w xh over the columns
-    float c[2 * ROWS];
+    constexpr int Q = 2 * ROWS;
+    float c[Q];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      c[2 * r] = c[2 * r + 1] = 0.f;
+      F2 s1 = 0ull, s2 = 0ull;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float gw = d[r][i][j] * w[i][j];
-          c[2 * r] += gw;
-          c[2 * r + 1] = fmaf(gw, xh[r][i][j], c[2 * r + 1]);
-          dw[i][j] = fmaf(d[r][i][j], xh[r][i][j], dw[i][j]);
-          db[i][j] += d[r][i][j];
+        for (int j = 0; j < V / 2; ++j) {
+          const F2 gw = mul2(d[r][i][j], w[i][j]);
+          s1 = add2(s1, gw);
+          s2 = fma2(gw, xh[r][i][j], s2);
+          dw[i][j] = fma2(d[r][i][j], xh[r][i][j], dw[i][j]);
+          db[i][j] = add2(db[i][j], d[r][i][j]);
+        }
+      c[r] = parts(s1).x + parts(s1).y;
+      c[ROWS + r] = parts(s2).x + parts(s2).y;
+    }
+    // Over the lanes: each step halves the sums that a lane keeps, until it has one of the Q, of 32 / Q lanes' values; lane l then has
+    // sum l / (32 / Q) of its warp.
+    int keep = Q / 2;
+#pragma unroll
+    for (int o = 16; o >= 32 / Q; o >>= 1, keep >>= 1) {
+      const bool upper = lane & o;
+#pragma unroll
+      for (int q = 0; q < Q / 2; ++q)
+        if (q < keep) {
+          const float away = upper ? c[q] : c[q + keep], mine = upper ? c[q + keep] : c[q];
+          c[q] = mine + __shfl_xor_sync(0xffffffffu, away, o);
         }
     }
 #pragma unroll
-    for (int q = 0; q < 2 * ROWS; ++q) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) c[q] += __shfl_xor_sync(0xffffffffu, c[q], o);
-    }
+    for (int o = 16 / Q; o > 0; o >>= 1) c[0] += __shfl_xor_sync(0xffffffffu, c[0], o);
+    float sum = c[0];
+    int per = 32 / Q;   // lane q * per has the row's sum q
     if (nw > 1) {
-      // the group's warps: lane q of each leaves its sum q, every warp adds them in the warps' order
-      float mine = c[0];
-#pragma unroll
-      for (int q = 1; q < 2 * ROWS; ++q)
-        if (lane == q) mine = c[q];
-      float* const room = s_all + buf * warps * 2 * ROWS;
-      if (lane < 2 * ROWS) room[warp * 2 * ROWS + lane] = mine;
+      // a group's warps, in an order of their own: lane l adds sum l % Q of every (32 / Q)th of them
+      float* const room = s_all + buf * warps * Q;
+      if (lane % per == 0) room[warp * Q + lane / per] = sum;
       __syncthreads();   // (two buffers: the next round's sums do not meet this one's readers)
-      float sum = 0.f;
-      if (lane < 2 * ROWS)
-        for (int i = 0; i < nw; ++i) sum += room[(g * nw + i) * 2 * ROWS + lane];
+      sum = 0.f;
+      for (int i = lane / Q; i < nw; i += 32 / Q) sum += room[(g * nw + i) * Q + lane % Q];
 #pragma unroll
-      for (int q = 0; q < 2 * ROWS; ++q) c[q] = __shfl_sync(0xffffffffu, sum, q);
+      for (int o = 16; o >= Q; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      per = 1;
     }
     if (p.dx == nullptr) continue;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int row = r0 + r;
+      const float c1 = -__shfl_sync(0xffffffffu, sum, r * per) * inv_k * rstd[r], c2 = -__shfl_sync(0xffffffffu, sum, (ROWS + r) * per) * inv_k * rstd[r];
       if (row >= p.M) continue;   // (whole warps)
       T* const out = static_cast<T*>(p.dx) + row * p.xs;
       const T* const more = p.dh ? static_cast<const T*>(p.dh) + row * p.ds : nullptr;
-      const float c1 = -c[2 * r] * inv_k * rstd[r], c2 = -c[2 * r + 1] * inv_k * rstd[r];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int k = t * V + i * step;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = fmaf(xh[r][i][j], c2, fmaf(d[r][i][j] * w[i][j], rstd[r], c1));
+        for (int j = 0; j < V / 2; ++j) {
+          const float2 u = parts(fma2(xh[r][i][j], pair_of(c2, c2), fma2(mul2(d[r][i][j], w[i][j]), pair_of(rstd[r], rstd[r]), pair_of(c1, c1))));
+          o[2 * j] = u.x;
+          o[2 * j + 1] = u.y;
+        }
         if (more) {
           float a[V];
           Num<T>::unpack(load_row<T, WHOLE>(more, k, K), a);
@@ -797,8 +847,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
       for (int j = 0; j < V; ++j) {
         const int k = t * V + i * step + j;
         if (k < K) {
-          mine[k] = dw[i][j];
-          mine[K + k] = db[i][j];
+          mine[k] = j & 1 ? parts(dw[i][j / 2]).y : parts(dw[i][j / 2]).x;
+          mine[K + k] = j & 1 ? parts(db[i][j / 2]).y : parts(db[i][j / 2]).x;
         }
       }
     __syncthreads();
@@ -815,8 +865,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
     for (int j = 0; j < V; ++j) {
       const int k = t * V + i * step + j;
       if (k < K) {
-        at[k] = dw[i][j];
-        at[K + k] = db[i][j];
+        at[k] = j & 1 ? parts(dw[i][j / 2]).y : parts(dw[i][j / 2]).x;
+        at[K + k] = j & 1 ? parts(db[i][j / 2]).y : parts(db[i][j / 2]).x;
       }
     }
 }
@@ -891,18 +941,19 @@ template <typename T> __global__ void __launch_bounds__(256) long_grad_kernel(co
 
 // How the gradients of [M, K] are cut: NV pieces a thread, ROWS rows at a time, groups of a CTA; NV = 0: rows that do not fit a CTA.
 struct GradPlan {
-  int nv, rows, group, groups, parts;
+  int nv, group, groups, rows, parts;
   size_t smem;
 };
 GradPlan grad_plan(int M, int K, int vec) {
   GradPlan g{};
   const int n = (K + vec - 1) / vec;
   g.nv = n <= kGradThreads ? 1 : n <= 2 * kGradThreads ? 2 : 0;
-  g.rows = g.nv == 1 ? 2 : 1;
   g.group = g.nv ? ((n + g.nv - 1) / g.nv + 31) / 32 * 32 : 256;
   g.groups = g.group >= 256 ? 1 : 256 / g.group;
-  const int per = g.nv ? g.rows * g.groups : 1;
-  g.parts = std::max(1, std::min(kGradParts, (M + per - 1) / per));
+  // two rows at a time in 128 registers and two CTAs to an SM, or one row in 64 and one CTA
+  g.rows = g.nv && g.group * g.groups <= 256 ? 2 : 1;
+  const int per = g.rows * g.groups;
+  g.parts = std::max(1, std::min(g.rows * (kGradParts / 2), g.nv ? (M + per - 1) / per : M / 16));
   const int warps = g.group * g.groups / 32;
   g.smem = std::max<size_t>(2ull * warps * 2 * g.rows, g.groups > 1 ? 2ull * g.groups * K : 0) * 4;
   return g;
@@ -930,8 +981,8 @@ template <typename T, bool WHOLE> cudaError_t launch_grad_of(GradParams p, cudaS
     cfg.attrs = attr;
     cfg.numAttrs = use_pdl() ? 1 : 0;
     e = g.nv == 2                    ? cudaLaunchKernelEx(&cfg, norm_grad_kernel<T, WHOLE, 2, 1, kGradThreads, 1>, p)
-        : g.group * g.groups <= 256 ? cudaLaunchKernelEx(&cfg, norm_grad_kernel<T, WHOLE, 1, 2, 256, 2>, p)
-                                    : cudaLaunchKernelEx(&cfg, norm_grad_kernel<T, WHOLE, 1, 2, kGradThreads, 1>, p);
+        : g.rows == 2                 ? cudaLaunchKernelEx(&cfg, norm_grad_kernel<T, WHOLE, 1, 2, 256, 2>, p)
+                                    : cudaLaunchKernelEx(&cfg, norm_grad_kernel<T, WHOLE, 1, 1, kGradThreads, 1>, p);
   }
   if (e != cudaSuccess || p.dweight == nullptr) return e;
   p.partial = room;

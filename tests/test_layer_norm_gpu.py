@@ -10,6 +10,12 @@ TYPES = [torch.float16, torch.bfloat16, torch.float32]
 EPS = 1e-5
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    w8.read_status()
+
+
 def inputs(m, k, dtype, residual=False, seed=0):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
@@ -49,7 +55,7 @@ def exact(h, w, b, dy=None, dh=None):
 
 
 SIZES = [(1, 1), (1, 8), (2, 7), (5, 96), (3, 1000), (1, 2048), (70, 2048), (9, 1023), (33, 5120), (1300, 64), (4, 12000), (2, 16384), (3, 18945),
-         (2, 40000), (601, 40)]
+         (2, 40000), (601, 40), (1200, 8), (700, 1027), (333, 6001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
