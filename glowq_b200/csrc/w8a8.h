@@ -17,6 +17,9 @@ bool use_pdl();
 
 // w8a8_rows.cu
 cudaError_t launch_rows(const glowq_w8a8_rows_t& p, int sms, cudaStream_t stream);
+// codes, scales and r of a few tokens in one launch
+bool few_tokens(const glowq_w8a8_linear_t& g);
+cudaError_t launch_few_tokens(const glowq_w8a8_linear_t& g, cudaStream_t stream);
 cudaError_t launch_layer_norm_grad(const glowq_layer_norm_grad_t& g, cudaStream_t stream);
 size_t layer_norm_grad_bytes(int M, int K);
 

@@ -147,19 +147,23 @@ int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
   if (rc != GLOWQ_OK || g.M == 0) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(g.stream);
   if (g.alpha == 0.f) g.r_mode = GLOWQ_R_NONE;   // nothing to add
-  if (g.x) {
-    glowq_w8a8_rows_t r{};
-    r.x = g.x;
-    r.x_stride = g.x_stride;
-    r.codes = g.codes;
-    r.code_stride = g.code_stride;
-    r.scales = g.scales;
-    r.M = g.M;
-    r.K = g.K;
-    r.dtype = g.x_dtype;
-    if ((rc = note_cuda_error(launch_rows(r, sms, stream))) != GLOWQ_OK) return rc;
+  if (g.x && g.r_mode == GLOWQ_R_COMPUTE && few_tokens(g)) {
+    if ((rc = note_cuda_error(launch_few_tokens(g, stream))) != GLOWQ_OK) return rc;
+  } else {
+    if (g.x) {
+      glowq_w8a8_rows_t r{};
+      r.x = g.x;
+      r.x_stride = g.x_stride;
+      r.codes = g.codes;
+      r.code_stride = g.code_stride;
+      r.scales = g.scales;
+      r.M = g.M;
+      r.K = g.K;
+      r.dtype = g.x_dtype;
+      if ((rc = note_cuda_error(launch_rows(r, sms, stream))) != GLOWQ_OK) return rc;
+    }
+    if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, true, sms, stream)) != GLOWQ_OK) return rc;
   }
-  if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, true, sms, stream)) != GLOWQ_OK) return rc;
   const int n = pair_columns(g, sms);
   return n > 0 ? w8a8_pair_forward(g, n, sms, stream) : w8a8_stream_forward(g, sms, stream);
 }

@@ -5,13 +5,13 @@
 //   y = s_t w_o D + alpha F + bias
 //
 // and, with fp16 operands in the first place, r = x . R^T (channels: the rows of R).
-//   Bound by HBM: every weight is read once.  TMA brings 128 rows x 128 bytes of weights and N tokens' 128 bytes a step into a ring of
-// 96 to 108 KB, two CTAs to an SM, and tcgen05.mma reads both from there: no weight passes through registers.  The weights do not hang
+//   Bound by HBM: every weight is read once.  TMA brings 128 rows x 128 bytes of weights and N tokens' 128 bytes a step into a ring
+// of 200 KB (or two CTAs to an SM, of 100 KB each), and tcgen05.mma reads both from there: no weight passes through registers.  The weights do not hang
 // on the kernels before, so the ring is filled before the dependency wait: a launch's first 30 MB of weights arrive while the codes are
-// still being made.  The steps of a tile are shared out over the CTAs of a cluster (up to 8) so that about two CTAs per SM
-// are at work whatever the number of channels; their sums meet in shared memory (each CTA reads its share of the others' blocks),
+// still being made.  The steps of a tile are shared out over the CTAs of a cluster (up to 8) so that all SMs are
+// at work whatever the number of channels; their sums meet in shared memory (each CTA reads its share of the others' blocks),
 // integers in any order, the correction's fp32 sums in the order of the CTAs: no workspace, no counters, the same bits every time.
-//   warp 0  copies (one thread)      warp 1  tensor memory, MMAs      warps 2-5  sums to shared memory; all: scales, bias, output
+//   warps 0 and 6  copies (a thread each)    warp 1  tensor memory, MMAs    warps 2-5  sums to shared memory; all: scales, bias, output
 // Tensor memory is taken after the dependency wait: a CTA that held it while it waits could keep a kernel in front from taking its own.
 #include <cuda_bf16.h>
 
@@ -28,9 +28,10 @@ __device__ uint32_t g_w8a8_status;   // nonzero once a wait of one of this file'
 
 constexpr int kRows = 128;
 constexpr int kAStage = kRows * 128;
-constexpr int kThreads = 192;
-constexpr int kSmemTwo = 113 * 1024;   // dynamic shared memory at most, two CTAs to an SM
-constexpr int kMaxStages = 8;
+constexpr int kThreads = 224;
+// Dynamic shared memory at most: of a launch whose CTAs have an SM each, and of one that has more of them, two to an SM.
+constexpr int kSmemOne = 220 * 1024, kSmemTwo = 113 * 1024;
+constexpr int kMaxStages = 12;
 constexpr int kMaxSplit = 8;
 constexpr unsigned kDrainSpin = 1u << 18;
 
@@ -47,8 +48,8 @@ struct alignas(64) StreamMaps {
   CUtensorMap a, b, l, r;
 };
 
-template <int N> constexpr int stages_of() { return std::min(kMaxStages, (kSmemTwo - 2048) / (kAStage + N * 128)); }
-template <int N> constexpr int smem_of() { return 2048 + stages_of<N>() * (kAStage + N * 128); }
+template <int N, bool TWO> constexpr int stages_of() { return std::min(kMaxStages, ((TWO ? kSmemTwo : kSmemOne) - 2048) / (kAStage + N * 128)); }
+template <int N, bool TWO> constexpr int smem_of() { return 2048 + stages_of<N, TWO>() * (kAStage + N * 128); }
 
 // The four MMAs of a step (32 bytes of K each) and the commit that gives its stage back, by one elected lane of a converged warp.
 #define GLOWQ_STREAM_STEP(KIND)                                                                                                     \
@@ -121,10 +122,11 @@ __device__ __forceinline__ void store4(const StreamParams& p, int token, int col
 }
 
 // N tokens a tile; F16: fp16 operands and fp32 sums (r = x . R^T, which has neither scales nor a correction).
-template <int N, bool F16>
-__global__ void __launch_bounds__(kThreads, 2) stream_kernel(const __grid_constant__ StreamParams p, const __grid_constant__ StreamMaps tm) {
-  constexpr int kStages = stages_of<N>(), kStage = kAStage + N * 128;
+template <int N, bool F16, bool TWO>
+__global__ void __launch_bounds__(kThreads, TWO ? 2 : 1) stream_kernel(const __grid_constant__ StreamParams p, const __grid_constant__ StreamMaps tm) {
+  constexpr int kStages = stages_of<N, TWO>(), kStage = kAStage + N * 128;
   constexpr uint32_t kFull = 0, kEmpty = 8 * kMaxStages, kAcc = 16 * kMaxStages;
+  static_assert(kAcc + 8 <= 1024, "barriers");
   extern __shared__ unsigned char smem[];
   __shared__ int s_abort;
   __shared__ uint32_t s_tmem;
@@ -150,28 +152,20 @@ __global__ void __launch_bounds__(kThreads, 2) stream_kernel(const __grid_consta
   __syncthreads();
   if (p.early && threadIdx.x == 64) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const auto load_a = [&](int it, int stage) {
-    const uint32_t bar = smem0 + kFull + 8 * stage, dst = ring + stage * kStage;
+  // The first steps' weights are asked for before the dependency wait.
+  const int ahead = min(kStages, it1 - it0);
+  const auto load_a = [&](int it, uint32_t bar, uint32_t dst) {
     g_mbar_expect_tx(bar, kStage);
     if (it < p.nk)
       g_tma_2d(dst, &tm.a, it * (F16 ? 64 : 128), n0, bar);
     else
       g_tma_2d(dst, &tm.l, (it - p.nk) * 64, n0, bar);
   };
-  const auto load_b = [&](int it, int stage) {
-    const uint32_t bar = smem0 + kFull + 8 * stage, dst = ring + stage * kStage + kAStage;
-    if (it < p.nk)
-      g_tma_2d(dst, &tm.b, it * (F16 ? 64 : 128), m0, bar);
-    else
-      g_tma_2d(dst, &tm.r, (it - p.nk) * 64, m0, bar);
-  };
-  const int ahead = min(kStages, it1 - it0);
   if (threadIdx.x == 0)
-    for (int i = 0; i < ahead; ++i) load_a(it0 + i, i);
+    for (int i = 0; i < ahead; ++i) load_a(it0 + i, smem0 + kFull + 8 * i, ring + i * kStage);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (threadIdx.x == 0)
-    for (int i = 0; i < ahead; ++i) load_b(it0 + i, i);
-  const uint32_t columns = p.nr > 0 ? (2 * N < 32 ? 32 : 2 * N) : (N < 32 ? 32 : N);
+  // (a constant: with a number of columns that the launch chose, an SM held one CTA instead of two)
+  constexpr uint32_t columns = F16 ? (N < 32 ? 32 : N) : 2 * N;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_u32(&s_tmem)), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -203,21 +197,31 @@ __global__ void __launch_bounds__(kThreads, 2) stream_kernel(const __grid_consta
   Scales mine{};
   if (!F16 && q_mine < q1) mine = scales_of(q_mine);
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 6) {
+    // Copies: warp 0 the weights (and L) and the announcement of a step's bytes, warp 6 the tokens (and r).  One thread for both took a
+    // thousand clocks a step: 43 GB/s of weights.
     if (lane == 0) {
-      int issued = ahead;
-      for (int it = it0 + ahead; it < it1; ++it, ++issued) {
-        const int stage = issued % kStages;
-        if (!g_mbar_wait(smem0 + kEmpty + 8 * stage, (issued / kStages + 1) & 1, abort_flag, status) || *abort_flag) break;
-        load_a(it, stage);
-        load_b(it, stage);
-      }
-      // the copies have landed before the CTA goes on
-      for (int j = max(0, issued - kStages); j < issued; ++j) {
-        uint32_t spins = 0;
-        while (!g_mbar_try_once(smem0 + kFull + 8 * (j % kStages), (j / kStages) & 1) && ++spins < kDrainSpin) {
+      const bool weights = warp == 0;
+      uint32_t stage = weights && ahead == kStages ? 0u : weights ? static_cast<uint32_t>(ahead) : 0u, ph = weights && ahead == kStages ? 0u : 1u;
+      for (int it = it0 + (weights ? ahead : 0); it < it1; ++it) {
+        const uint32_t bar = smem0 + kFull + 8 * stage, dst = ring + stage * kStage;
+        if (!g_mbar_wait(smem0 + kEmpty + 8 * stage, ph, abort_flag, status)) break;
+        if (weights)
+          load_a(it, bar, dst);
+        else
+          g_tma_2d(dst + kAStage, it < p.nk ? &tm.b : &tm.r, it < p.nk ? it * (F16 ? 64 : 128) : (it - p.nk) * 64, m0, bar);
+        if (++stage == kStages) {
+          stage = 0;
+          ph ^= 1;
         }
       }
+      // the copies have landed before the CTA goes on (or the wait for them runs out)
+      if (weights)
+        for (int j = max(0, it1 - it0 - kStages); j < it1 - it0; ++j) {
+          uint32_t spins = 0;
+          while (!g_mbar_try_once(smem0 + kFull + 8 * (j % kStages), (j / kStages) & 1) && ++spins < kDrainSpin) {
+          }
+        }
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_kernel(const __grid_consta
   }
   // sums of a CTA: [tokens][128] of the product, then of the correction, where the ring was
   const uint32_t sums = ring;
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const bool ok = __all_sync(0xffffffffu, g_mbar_wait(smem0 + kAcc, 0, abort_flag, status));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
@@ -323,26 +327,34 @@ __global__ void __launch_bounds__(kThreads, 2) stream_kernel(const __grid_consta
   if (split > 1) cluster_sync_all();   // the others' reads of this CTA's sums
 }
 
-template <int N, bool F16>
+// CTAs of a cluster: as many as leave all tiles in one round with an SM for each CTA (clusters of some sizes fill the SMs less well), each
+// with two steps at least.  us, one token, 5120 -> 5120 (40 tiles) in clusters of 1, 2, 3, 4: 10.1, 8.4, 7.4, 11.8; 77 tokens,
+// 18944 -> 3584 (28 tiles) in 1 to 5: 37.5, 23.3, 19.3, 17.2, 28.9.
+int plan_split(long long tiles, int steps, int sms) {
+  constexpr int kHeld[kMaxSplit + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};   // CTAs in clusters of 1 to 8 on 148 SMs
+  int best = 1;
+  for (int s = 2; s <= std::min(kMaxSplit, steps / 2); ++s)
+    if (tiles * s <= static_cast<long long>(kHeld[s]) * sms / 148) best = s;
+  return best;
+}
+
+template <int N, bool F16, bool TWO>
 int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t stream) {
-  static_assert((F16 ? 1 : N <= 64 ? 2 : 1) * N * kRows * 4 <= smem_of<N>() - 2048, "the sums fit the ring");
+  constexpr int smem = smem_of<N, TWO>();
   const int x = (p.OC + kRows - 1) / kRows, y = (p.M + N - 1) / N;
-  // CTAs of a cluster: as many as two to an SM allow, each with two steps at least
-  const long long tiles = static_cast<long long>(x) * y;
-  const int room = static_cast<int>(std::min<long long>(kMaxSplit, std::max<long long>(1, 2 * sms / tiles)));
-  p.split = std::max(1, std::min(room, (p.nk + p.nr) / 2));
+  p.split = TWO ? 1 : plan_split(static_cast<long long>(x) * y, p.nk + p.nr, sms);
   static bool attr_done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<N, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of<N>());
+    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<N, F16, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return note_cuda_error(e);
     attr_done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(x * p.split, y);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_of<N>();
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -358,13 +370,23 @@ int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t st
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return note_cuda_error(cudaLaunchKernelEx(&cfg, stream_kernel<N, F16>, p, tm));
+  return note_cuda_error(cudaLaunchKernelEx(&cfg, stream_kernel<N, F16, TWO>, p, tm));
+}
+template <int N, bool F16> int launch_ring(const StreamParams& p, const StreamMaps& tm, int sms, cudaStream_t stream) {
+  static_assert((F16 ? 1 : 2) * N * kRows * 4 <= smem_of<N, false>() - 2048, "the sums fit the ring");
+  // Two CTAs to an SM where one each would leave a second round: 16 tokens, 5120 -> 27648 (216 tiles) 25.5 us, so 29.3; with one round
+  // the deeper ring: 5120 -> 13824 (108 tiles) 13.1 us, so 14.7.  (Their rings do not hold the two blocks of sums of 128 tokens.)
+  if constexpr (N <= 64) {
+    static_assert((F16 ? 1 : 2) * N * kRows * 4 <= smem_of<N, true>() - 2048, "the sums fit the ring");
+    if (static_cast<long long>((p.OC + kRows - 1) / kRows) * ((p.M + N - 1) / N) > sms) return launch_stream<N, F16, true>(p, tm, sms, stream);
+  }
+  return launch_stream<N, F16, false>(p, tm, sms, stream);
 }
 template <bool F16> int launch_tokens(const StreamParams& p, const StreamMaps& tm, int n, int sms, cudaStream_t stream) {
-  if (n == 16) return launch_stream<16, F16>(p, tm, sms, stream);
-  if (n == 32) return launch_stream<32, F16>(p, tm, sms, stream);
-  if (n == 64) return launch_stream<64, F16>(p, tm, sms, stream);
-  return launch_stream<128, F16>(p, tm, sms, stream);
+  if (n == 16) return launch_ring<16, F16>(p, tm, sms, stream);
+  if (n == 32) return launch_ring<32, F16>(p, tm, sms, stream);
+  if (n == 64) return launch_ring<64, F16>(p, tm, sms, stream);
+  return launch_ring<128, F16>(p, tm, sms, stream);
 }
 
 }  // namespace
@@ -373,7 +395,7 @@ cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream) { return take
 
 int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stream) {
   const bool corrected = g.r_mode != GLOWQ_R_NONE;
-  const int n = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 || corrected ? 64 : 128;
+  const int n = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   StreamParams p{};
   p.scales = g.scales;
   p.weight_scales = g.weight_scales;

@@ -28,18 +28,26 @@ class TokenCodes(NamedTuple):
     r: Optional[torch.Tensor] = None
 
 
+# (Small calls cost what the host does: sizes in the place of a tuple and a known device take a third off an allocation, 0.8 us.)
+_empty, _int8, _float32, _float16 = torch.empty, torch.int8, torch.float32, torch.float16
+
+
 def _pitch(k: int) -> int:
     return (k + 15) & ~15
 
 
 def _new_codes(m: int, k: int, device) -> torch.Tensor:
-    pitch = _pitch(k)
-    t = torch.empty((m, pitch), dtype=torch.int8, device=device)
+    pitch = (k + 15) & ~15
+    t = _empty(m, pitch, dtype=_int8, device=device)
     return t if pitch == k else t[:, :k]
 
 
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """``x`` as [rows, columns] with unit column stride and rows that do not overlap."""
+    if x.is_cuda and x.dtype in K.DTYPES and x.dim() == 2:      # (mostly all is well)
+        (m, k), (s0, s1) = x.shape, x.stride()
+        if s1 == 1 and k > 0 and (s0 >= k or m <= 1):
+            return x
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be CUDA (sm_100); there is no CPU path")
     if x.dtype not in K.DTYPES:
@@ -56,23 +64,22 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     return x
 
 
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the copy engine reads it: rows that begin on 16 bytes.  (Others are copied; what the package makes lies so.)"""
-    e = t.element_size()
-    stride = t.stride()
-    if t.data_ptr() % 16 == 0 and (stride[1] == 1 or t.shape[1] == 1) and (
-            t.shape[0] <= 1 or (stride[0] * e % 16 == 0 and stride[0] >= t.shape[1])):
-        return t
-    cols = 16 // e
-    room = torch.empty((t.shape[0], (t.shape[1] + cols - 1) // cols * cols), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
-    room.copy_(t)
-    return room
-
-
-def _operand_stride(t: torch.Tensor) -> int:
-    """(of a single row the stride may be anything; the library is told one that it accepts)"""
-    cols = 16 // t.element_size()
-    return t.stride()[0] if t.shape[0] > 1 else (t.shape[1] + cols - 1) // cols * cols
+def _place(t: torch.Tensor, e: int):
+    """(tensor, address, row stride) of a matrix of ``e``-byte elements as the copy engine reads it: rows that begin on 16 bytes.  (Others
+    are copied; what the package makes lies so.  Of a single row the stride may be anything: the library is told one that it accepts.)"""
+    at, (rows, cols), (s0, s1) = t.data_ptr(), t.shape, t.stride()
+    if not at & 15 and s1 == 1:
+        if rows > 1:
+            if s0 >= cols and not s0 * e & 15:
+                return t, at, s0
+        else:
+            per = 16 // e
+            return t, at, (cols + per - 1) // per * per
+    per = 16 // e
+    pitch = (cols + per - 1) // per * per
+    room = _empty(rows, pitch, dtype=t.dtype, device=t.device)
+    room[:, :cols].copy_(t)
+    return room, room.data_ptr(), pitch
 
 
 def _quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, constant: bool) -> None:
@@ -83,10 +90,10 @@ def _quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, consta
 
 def quantize_tokens(x: torch.Tensor) -> TokenCodes:
     """int8 codes and a scale for every row of ``x`` [..., in_features] (fp16, bf16 or fp32), in one launch."""
-    x = _rows(x.detach(), "x")
-    m, k = x.shape
-    codes = _new_codes(m, k, x.device)
-    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    x = _rows(x, "x")
+    (m, k), dev = x.shape, x.device
+    codes = _new_codes(m, k, dev)
+    scales = _empty(m, dtype=_float32, device=dev)
     if m:
         _quantize(x, codes, scales, False)
     return TokenCodes(codes, scales)
@@ -104,7 +111,8 @@ def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
     if oc == 0:
         return codes, scales
     if weight.is_cuda:
-        _quantize(_rows(weight, "weight"), codes, scales, True)
+        weight = _rows(weight, "weight")
+        _quantize(weight, codes, scales, True)
         return codes, scales
     top = weight.float().abs().amax(dim=1)
     torch.div(top, torch.full_like(top, 127.0), out=scales)
@@ -127,47 +135,51 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
         raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
     if kind == K.NORM_RMS and bias is not None:
         raise ValueError("RMSNorm has no bias")
-    x2 = _rows(x.detach(), "x")
-    m, k = x2.shape
+    x2 = _rows(x, "x")
+    (m, k), dev = x2.shape, x2.device
     check_norm(x2, weight, bias, eps)
-    res, hidden = residual, x
+    res_at = res_stride = hid_at = 0
+    hidden = x
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
             raise RuntimeError("residual must have x's shape, type and device")
-        res = _rows(residual.detach(), "residual")
-        hidden = torch.empty((m, k), dtype=x.dtype, device=x.device)
-    codes = _new_codes(m, k, x.device)
-    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+        res = _rows(residual, "residual")
+        hidden = _empty(m, k, dtype=x.dtype, device=dev)
+        res_at, res_stride, hid_at = res.data_ptr(), res.stride()[0], hidden.data_ptr()
+    codes = _new_codes(m, k, dev)
+    scales = _empty(m, dtype=_float32, device=dev)
     if m:
-        w = weight.detach().contiguous()
-        b = bias.detach().contiguous() if bias is not None else None
-        with_res = res is not None
-        desc = _pack_rows(x2.data_ptr(), res.data_ptr() if with_res else 0, w.data_ptr(), b.data_ptr() if b is not None else 0,
-                          hidden.data_ptr() if with_res else 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0,
-                          current_stream_ptr(x.device), float(eps), x2.stride()[0], res.stride()[0] if with_res else 0, k, 0,
-                          codes.stride()[0], m, k, K.DTYPES[x.dtype], kind, 0, 0)
-        K.call(K.ext().quantize, x.device, desc, "glowq_w8a8_quantize")
-    if residual is not None:
+        weight = weight.contiguous()
+        b_at = 0
+        if bias is not None:
+            bias = bias.contiguous()
+            b_at = bias.data_ptr()
+        desc = _pack_rows(x2.data_ptr(), res_at, weight.data_ptr(), b_at, hid_at, 0, codes.data_ptr(), scales.data_ptr(), 0, 0,
+                          current_stream_ptr(dev), eps, x2.stride()[0], res_stride, k, 0, codes.stride()[0], m, k, K.DTYPES[x2.dtype], kind,
+                          0, 0)
+        K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
+    if residual is not None and x.dim() != 2:
         hidden = hidden.reshape(x.shape)
     return TokenCodes(codes, scales), hidden
 
 
 def check_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
     """(``x``: what ``_rows`` gave)"""
-    k = x.shape[1]
+    k, dtype, dev = x.shape[1], x.dtype, x.device
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None and name == "bias":
             continue
-        if t is None or t.dim() != 1 or t.shape[0] != k or t.dtype != x.dtype or t.device != x.device:
+        if t is None or t.dtype != dtype or t.device != dev or t.dim() != 1 or t.shape[0] != k:
             raise RuntimeError(f"{name} must be [{k}] of x's type on x's device")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
 
 
-def _factor(t: torch.Tensor, name: str, rows: int, cols: Optional[int], device) -> torch.Tensor:
-    if t.dim() != 2 or t.dtype != torch.float16 or t.device != device or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
+def _factor(t: torch.Tensor, name: str, rows: int, cols: Optional[int], device):
+    """(``_place`` of a factor)"""
+    if t.dtype != _float16 or t.device != device or t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
         raise RuntimeError(f"{name} must be fp16 [{rows}, {'rank' if cols is None else cols}] on {device}, got {t.dtype} {tuple(t.shape)}")
-    return _operand(t.detach())
+    return _place(t.detach() if t.requires_grad else t, 2)
 
 
 def right_factor(x: torch.Tensor, R: torch.Tensor) -> torch.Tensor:
@@ -176,16 +188,19 @@ def right_factor(x: torch.Tensor, R: torch.Tensor) -> torch.Tensor:
     x = _rows(x.detach(), "x")
     if R.dim() != 2 or not 0 < R.shape[0] <= K.MAX_RANK:
         raise RuntimeError(f"R must be [rank, in_features] with a rank of 1 to {K.MAX_RANK}")
-    m, k = x.shape
-    R = _factor(R, "R", R.shape[0], k, x.device)
+    (m, k), dev = x.shape, x.device
+    if m > K.MAX_TOKENS:
+        raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
+    R, R_at, R_stride = _factor(R, "R", R.shape[0], k, dev)
     rank = R.shape[0]
-    r = torch.empty((m, (rank + 7) & ~7), dtype=torch.float16, device=x.device)[:, :rank]
+    pitch = (rank + 7) & ~7
+    r = _empty(m, pitch, dtype=_float16, device=dev)
     if m:
-        x = _operand(x if x.dtype == torch.float16 else x.to(torch.float16))
-        desc = _pack_linear(0, 0, 0, 0, 0, 0, x.data_ptr(), R.data_ptr(), r.data_ptr(), 0, 0, current_stream_ptr(x.device), 0, 0, 0,
-                            _operand_stride(x), _operand_stride(R), _operand_stride(r), 0, 0, m, k, 0, rank, 0, 0, K.R_COMPUTE, 0.0, 0)
-        K.call(K.ext().right_factor, x.device, desc, "glowq_w8a8_right_factor")
-    return r
+        x, x_at, x_stride = _place(x if x.dtype == _float16 else x.to(_float16), 2)
+        desc = _pack_linear(0, 0, 0, 0, 0, 0, x_at, R_at, r.data_ptr(), 0, 0, current_stream_ptr(dev), 0, 0, 0, x_stride, R_stride, pitch, 0,
+                            0, m, k, 0, rank, 0, 0, K.R_COMPUTE, 0.0, 0)
+        K.call(K.ext().right_factor, dev, desc, "glowq_w8a8_right_factor")
+    return r if pitch == rank else r[:, :rank]
 
 
 def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight_scales: torch.Tensor,
@@ -195,24 +210,23 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
     [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, fp16 for codes.  ``L`` fp16 [out_features, rank]:
     the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``."""
+    x2 = lead = r = None
     if isinstance(x, TokenCodes):
-        codes, scales, r = x.codes, x.scales, x.r
-        if not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2:
+        codes, scales, r = x
+        if not codes.is_cuda or codes.dtype != _int8 or codes.dim() != 2:
             raise RuntimeError("codes must be int8 [tokens, in_features] on a CUDA device")
-        m, k = codes.shape
-        dev = codes.device
-        if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != m or scales.device != dev:
+        (m, k), dev = codes.shape, codes.device
+        if scales.dtype != _float32 or scales.dim() != 1 or scales.shape[0] != m or scales.device != dev:
             raise RuntimeError(f"scales must be fp32 [{m}] on {dev}")
-        codes, scales = _operand(codes), scales.contiguous()
-        x2, lead = None, None
         if R is not None:
             raise RuntimeError("codes have no right factor's product to be made from: pass TokenCodes.r (right_factor(x, R))")
         if out_dtype is None:
-            out_dtype = torch.float16
+            out_dtype = _float16
     else:
-        x2, r = _rows(x.detach(), "x"), None
-        m, k = x2.shape
-        dev, lead = x2.device, x.shape
+        x2 = _rows(x, "x")
+        (m, k), dev = x2.shape, x2.device
+        if x.dim() != 2:
+            lead = x.shape[:-1]
         if (L is None) != (R is None):
             raise RuntimeError("a correction needs L and R")
         if out_dtype is None:
@@ -220,56 +234,59 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     out_code = K.DTYPES.get(out_dtype)
     if out_code is None:
         raise RuntimeError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
-    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.device != dev:
+    if weight.dtype != _int8 or weight.dim() != 2 or weight.device != dev:
         raise RuntimeError(f"weight must be int8 [out_features, in_features] on {dev}")
-    if weight.shape[1] != k:
-        raise ValueError(f"Input dim mismatch: got {k}, expected {weight.shape[1]}")
+    oc, ic = weight.shape
+    if ic != k:
+        raise ValueError(f"Input dim mismatch: got {k}, expected {ic}")
     if not 0 < k <= K.MAX_EXACT_K:
         raise RuntimeError(f"in_features must be 1 to {K.MAX_EXACT_K} (sums are exact in 32 bits)")
-    oc = weight.shape[0]
     for t, name in ((weight_scales, "weight_scales"), (bias, "bias")):
-        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != oc or t.device != dev):
+        if t is not None and (t.dtype != _float32 or t.dim() != 1 or t.shape[0] != oc or t.device != dev):
             raise RuntimeError(f"{name} must be fp32 [{oc}] on {dev}")
     if m > K.MAX_TOKENS:
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
-    out = torch.empty((m, oc), dtype=out_dtype, device=dev)
+    out = _empty(m, oc, dtype=out_dtype, device=dev)
     if m and oc:
-        weight, weight_scales = _operand(weight), weight_scales.contiguous()
-        bias = bias.detach().contiguous() if bias is not None else None
-        rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = 0
+        weight, w_at, w_stride = _place(weight, 1)
+        weight_scales = weight_scales.contiguous()
+        b_at = 0
+        if bias is not None:
+            bias = bias.contiguous()
+            b_at = bias.data_ptr()
+        rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = x_at = x_stride = x_code = 0
         if L is not None:
-            L = _factor(L, "L", oc, None, dev)
-            rank = L.shape[1]
+            rank = L.shape[1] if L.dim() == 2 else 0
+            L, L_at, L_stride = _factor(L, "L", oc, None, dev)
             if not 0 < rank <= K.MAX_RANK:
                 raise RuntimeError(f"the rank must be 1 to {K.MAX_RANK}")
-            L_at, L_stride = L.data_ptr(), _operand_stride(L)
             if x2 is None:
                 if r is None:
                     raise RuntimeError("a corrected linear of codes needs TokenCodes.r (right_factor(x, R))")
-                r = _factor(r, "r", m, rank, dev)
-                mode, r_at, r_stride = K.R_LOAD, r.data_ptr(), _operand_stride(r)
+                r, r_at, r_stride = _factor(r, "r", m, rank, dev)
+                mode = K.R_LOAD
             else:
-                R = _factor(R, "R", rank, k, dev)
-                rx = _operand(x2 if x2.dtype == torch.float16 else x2.to(torch.float16))
-                mode, R_at, R_stride, rx_at, rx_stride = K.R_COMPUTE, R.data_ptr(), _operand_stride(R), rx.data_ptr(), _operand_stride(rx)
-        x_at = x_stride = x_code = 0
+                R, R_at, R_stride = _factor(R, "R", rank, k, dev)
+                rx, rx_at, rx_stride = _place((x2 if x2.dtype == _float16 else x2.to(_float16)).detach(), 2)
+                mode = K.R_COMPUTE
         if x2 is None:
-            code_at, code_stride, scale_at = codes.data_ptr(), _operand_stride(codes), scales.data_ptr()
+            codes, code_at, code_stride = _place(codes, 1)
+            scales = scales.contiguous()
+            scale_at = scales.data_ptr()
         else:
             # codes, scales and r of this call: one piece of memory
             x_at, x_stride, x_code = x2.data_ptr(), x2.stride()[0], K.DTYPES[x2.dtype]
-            code_stride, r_stride = _pitch(k), (rank + 7) & ~7
+            code_stride, r_stride = (k + 15) & ~15, (rank + 7) & ~7
             scale_off = m * code_stride
             r_off = scale_off + (4 * m + 15 & ~15)
-            room = torch.empty(r_off + 2 * m * r_stride, dtype=torch.uint8, device=dev)
+            room = _empty(r_off + 2 * m * r_stride, dtype=_int8, device=dev)
             code_at = room.data_ptr()
             scale_at, r_at = code_at + scale_off, code_at + r_off
-        desc = _pack_linear(x_at, code_at, scale_at, weight.data_ptr(), weight_scales.data_ptr(), bias.data_ptr() if bias is not None else 0,
-                            rx_at, R_at, r_at, L_at, out.data_ptr(), current_stream_ptr(dev), x_stride, code_stride,
-                            _operand_stride(weight), rx_stride, R_stride, r_stride, L_stride, oc, m, k, oc, rank, x_code, out_code, mode,
-                            float(alpha), 0)
+        desc = _pack_linear(x_at, code_at, scale_at, w_at, weight_scales.data_ptr(), b_at, rx_at, R_at, r_at, L_at, out.data_ptr(),
+                            current_stream_ptr(dev), x_stride, code_stride, w_stride, rx_stride, R_stride, r_stride, L_stride, oc, m, k, oc,
+                            rank, x_code, out_code, mode, alpha, 0)
         K.call(K.ext().linear, dev, desc, "glowq_w8a8_linear")
-    return out if lead is None or len(lead) == 2 else out.reshape(*lead[:-1], oc)
+    return out if lead is None else out.reshape(*lead, oc)
 
 
 def read_status(device: Optional[torch.device] = None) -> None:

@@ -80,9 +80,12 @@ def ext() -> _Ext:
     return _ext
 
 
+_device_now = K.current_device
+
+
 def call(fn, device: torch.device, desc: bytes, what: str) -> None:
     """``fn(desc)`` with ``device`` current."""
-    if K.current_device() == device.index:
+    if _device_now() == device.index:
         rc = fn(desc)
     else:
         with torch.cuda.device(device):

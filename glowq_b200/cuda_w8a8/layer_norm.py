@@ -12,23 +12,24 @@ import torch.nn as nn
 
 from ..cuda_w4a16.kernels import current_stream_ptr
 from . import kernels as K
-from .functional import _rows, check_norm
+from .functional import _empty, _float32, _pack_rows, _rows, check_norm
 
 
 def _forward(x2, res, weight, bias, eps, statistics: bool):
-    m, k = x2.shape
-    dev = x2.device
-    y = torch.empty((m, k), dtype=x2.dtype, device=dev)
-    hidden = torch.empty((m, k), dtype=x2.dtype, device=dev) if res is not None else None
-    mean = torch.empty(m, dtype=torch.float32, device=dev) if statistics else None
-    rstd = torch.empty(m, dtype=torch.float32, device=dev) if statistics else None
+    (m, k), dev, dtype = x2.shape, x2.device, x2.dtype
+    y = _empty(m, k, dtype=dtype, device=dev)
+    hidden = mean = rstd = None
+    res_at = res_stride = hid_at = mean_at = rstd_at = 0
+    if res is not None:
+        hidden = _empty(m, k, dtype=dtype, device=dev)
+        res_at, res_stride, hid_at = res.data_ptr(), res.stride()[0], hidden.data_ptr()
+    if statistics:
+        mean, rstd = _empty(m, dtype=_float32, device=dev), _empty(m, dtype=_float32, device=dev)
+        mean_at, rstd_at = mean.data_ptr(), rstd.data_ptr()
     if m:
-        with_res = res is not None
-        desc = K.pack_rows.pack(x2.data_ptr(), res.data_ptr() if with_res else 0, weight.data_ptr(),
-                                bias.data_ptr() if bias is not None else 0, hidden.data_ptr() if with_res else 0, y.data_ptr(), 0, 0,
-                                mean.data_ptr() if statistics else 0, rstd.data_ptr() if statistics else 0, current_stream_ptr(dev),
-                                eps, x2.stride()[0], res.stride()[0] if with_res else 0, k, k, 0, m, k, K.DTYPES[x2.dtype],
-                                K.NORM_LAYER, 0, 0)
+        desc = _pack_rows(x2.data_ptr(), res_at, weight.data_ptr(), bias.data_ptr() if bias is not None else 0, hid_at, y.data_ptr(), 0, 0,
+                          mean_at, rstd_at, current_stream_ptr(dev), eps, x2.stride()[0], res_stride, k, k, 0, m, k, K.DTYPES[dtype],
+                          K.NORM_LAYER, 0, 0)
         K.call(K.ext().layer_norm_forward, dev, desc, "glowq_layer_norm_forward")
     return y, hidden, mean, rstd
 
@@ -36,8 +37,8 @@ def _forward(x2, res, weight, bias, eps, statistics: bool):
 def _backward(h, dy, dh, weight, mean, rstd, need_dx: bool, need_dw: bool):
     m, k = h.shape
     dev = h.device
-    dx = torch.empty((m, k), dtype=h.dtype, device=dev) if need_dx else None
-    dw, db = (torch.empty((2, k), dtype=h.dtype, device=dev).unbind(0) if need_dw else (None, None))
+    dx = _empty(m, k, dtype=h.dtype, device=dev) if need_dx else None
+    dw, db = (_empty(k, dtype=h.dtype, device=dev), _empty(k, dtype=h.dtype, device=dev)) if need_dw else (None, None)
     need = K.ext().lib.glowq_layer_norm_workspace_bytes(m, k)
     room = torch.empty(need, dtype=torch.uint8, device=dev)
     if not need_dx:
@@ -97,7 +98,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                                     or (residual is not None and residual.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, residual, float(eps))
     res = _rows(residual, "residual") if residual is not None else None
-    y, hidden, _, _ = _forward(x2, res, weight.contiguous(), bias.contiguous() if bias is not None else None, float(eps), False)
+    y, hidden, _, _ = _forward(x2, res, weight.contiguous(), bias.contiguous() if bias is not None else None, eps, False)
     if x.dim() != 2:
         y = y.reshape(x.shape)
         hidden = hidden.reshape(x.shape) if hidden is not None else None
