@@ -13,8 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libglowq_w4a16.so")
 SOURCES = ["abi.cu", "gemv_stream.cu", "dequant.cu", "gemm.cu", "tp_allreduce.cu", "r_product.cu", "quantize.cu", "gemm_tmem.cu", "gemm_pair.cu",
-           "w8a8_abi.cu", "w8a8_rows.cu", "w8a8_stream.cu", "w8a8_pair.cu"]
-HEADERS = ["common.cuh", "params.h", "tcgen05.cuh", "w8a8.h", os.path.join("..", "..", "include", "glowq_w4a16.h"),
+           "w8a8_abi.cu", "w8a8_rows.cu", "w8a8_rows_f16.cu", "w8a8_rows_bf16.cu", "w8a8_rows_f32.cu", "w8a8_stream.cu", "w8a8_pair.cu"]
+HEADERS = ["common.cuh", "params.h", "tcgen05.cuh", "w8a8.h", "w8a8_rows.cuh", os.path.join("..", "..", "include", "glowq_w4a16.h"),
            os.path.join("..", "..", "include", "glowq_w8a8.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]

@@ -19,6 +19,8 @@ import torch.nn as nn
 
 from .cuda_w4a16 import kernels as K
 from .cuda_w4a16.linear import CudaW4A16Linear
+from .cuda_w8a8.functional import TokenCodes
+from .cuda_w8a8.linear import CudaW8A8Linear
 
 try:  # tqdm only decorates the patch loop, as in the reference
     from tqdm import tqdm as _tqdm
@@ -275,13 +277,17 @@ class GroupLauncher:
 
 
 class AddSVDCorrection(nn.Module):
-    """``inner(x) + alpha_svd * (x B_q^T) A_q^T`` (src/step3_eval_dataset.py:450-516), fused into one launch."""
+    """``inner(x) + alpha_svd * (x B_q^T) A_q^T`` (src/step3_eval_dataset.py:450-516), fused into one launch.
+
+    ``inner`` may be a ``CudaW8A8Linear`` as well: a call then makes the codes of x, r = x B_q^T and the product of its own, and takes nothing
+    from an earlier one.  Members of a group share that work where the caller says so: ``tokens(x)`` of one of them gives ``TokenCodes``
+    that all take in the place of x."""
 
     def __init__(self, inner: nn.Module, A_q: torch.Tensor, B_q: torch.Tensor, role: str, is_group: bool,
                  group_cache: Optional[MiniGroupCache], alpha_svd: float = 1.0):
         super().__init__()
-        if not isinstance(inner, CudaW4A16Linear):
-            raise TypeError("AddSVDCorrection wraps CudaW4A16Linear modules only (no Triton / dense backends here)")
+        if not isinstance(inner, (CudaW4A16Linear, CudaW8A8Linear)):
+            raise TypeError("AddSVDCorrection wraps CudaW4A16Linear and CudaW8A8Linear modules only (no Triton / dense backends here)")
         self.inner = inner
         self.register_buffer("A_q", A_q.to(torch.float16).contiguous(), persistent=False)
         self.register_buffer("B_q", B_q.to(torch.float16).contiguous(), persistent=False)
@@ -304,7 +310,22 @@ class AddSVDCorrection(nn.Module):
             self._own_r = K.RRows()
         return self._own_r.rows(m, rank, device)
 
+    def tokens(self, x: torch.Tensor) -> TokenCodes:
+        """``x`` as the 8-bit members of this module's group take it: codes, and r with the group's right factor."""
+        inner = _inner(self)
+        if not isinstance(inner, CudaW8A8Linear):
+            raise TypeError("token codes are what CudaW8A8Linear modules take")
+        return inner.tokens(x, None if self._mismatch else self.B_q)
+
+    def _forward_w8a8(self, inner: CudaW8A8Linear, x) -> torch.Tensor:
+        if self.alpha_svd == 0.0 or self._mismatch:
+            return inner(x)
+        return inner.launch(x, L=self.A_q, R=None if isinstance(x, TokenCodes) else self.B_q, alpha=float(self.alpha_svd))
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        inner = _inner(self)
+        if isinstance(inner, CudaW8A8Linear):
+            return self._forward_w8a8(inner, x)
         gl = self.group_launcher
         if gl is not None and gl.usable and x.is_cuda:
             if gl._refs[0]() is self:
@@ -396,14 +417,15 @@ def _patch(model, shared, bmap, alpha_svd, groups_to_patch: Optional[Set[str]], 
                 print(f"AttributeError for {module_name}: {exc}")
             skipped += 1
             continue
-        if not isinstance(inner, CudaW4A16Linear):
+        if not isinstance(inner, (CudaW4A16Linear, CudaW8A8Linear)):
             skipped += 1
             continue
-        dev = inner.qweight_i32.device
+        dev = inner.scales_f32.device if isinstance(inner, CudaW8A8Linear) else inner.qweight_i32.device
         wrapper = AddSVDCorrection(inner, A_q.to(dev), B_q.to(dev), role=role, is_group=is_group,
                                    group_cache=cache, alpha_svd=alpha_svd)
         setattr(parent, leaf, wrapper)
-        wrapped.append((gkey, wrapper))
+        if isinstance(inner, CudaW4A16Linear):      # (launchers join the members of 4-bit groups)
+            wrapped.append((gkey, wrapper))
         patched += 1
     if verbose:
         print(f"SVD Correction Patching Summary: {patched} patched, {skipped} skipped")
