@@ -24,8 +24,10 @@ cudaError_t launch_layer_norm_grad(const glowq_layer_norm_grad_t& g, cudaStream_
 size_t layer_norm_grad_bytes(int M, int K);
 
 // w8a8_stream.cu
+int w8a8_stream_split(long long tiles, int steps, int sms);   // CTAs of a cluster
 int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stream);
-int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool early, int sms, cudaStream_t stream);
+// beside: the launch in front makes the codes of the same x, and began after all that came before it was complete
+int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, int sms, cudaStream_t stream);
 cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream);
 
 // w8a8_pair.cu: tiles of 256 tokens x n channels (64, 128, 192 or 256)

@@ -1,6 +1,6 @@
 // Entry points declared in include/glowq_w8a8.h: checks of the arguments and dispatch.
+#include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "w8a8.h"
 
@@ -83,20 +83,38 @@ int check_linear(const glowq_w8a8_linear_t& g) {
   return rc;
 }
 
+// Microseconds of a call of more than 64 tokens in either form (for choosing between them), on B200: fitted to eight weights from
+// 3584 x 1024 to 5120 x 27648 at 65 to 1024 tokens; within some 10 %.  (us, streaming / pairs of the width taken: 96 tokens 18944 -> 3584
+// 19.4 / 36.9, 5120 -> 27648 42.5 / 33.0; 200 tokens 18944 -> 3584 27.0 / 37.7, 5120 -> 13824 38.6 / 20.9.)
+// Streaming: rounds of CTAs, each a chain of about 6 to 8 us and its steps, which take 0.25 us or what HBM needs for all CTAs' weights.
+double stream_us(int M, long long steps, int OC, int sms) {
+  const long long x = (OC + 127) / 128, y = (M + 127) / 128, tiles = x * y;
+  const int split = w8a8_stream_split(tiles, static_cast<int>(steps), sms);
+  const double chain = 6.0 + 0.015 * std::min(M, 128), each = static_cast<double>((steps + split - 1) / split);
+  const auto round = [&](double ctas) { return chain + each * std::max(0.25, ctas * 16384.0 / 5.4e6); };
+  const long long ctas = tiles * split, whole = ctas / sms, rest = ctas % sms;
+  return static_cast<double>(whole) * round(sms) + (rest ? round(static_cast<double>(rest)) : 0.0);
+}
+// Pairs: a chain of 5.5 us, and rounds of tiles whose steps take what the narrow ones' copies or the wide ones' MMAs do.
+double pair_us(int M, long long steps, int OC, int n, int sms) {
+  const double step = n == 64 ? 0.211 : n == 128 ? 0.224 : n == 192 ? 0.228 : 0.292;
+  const long long tiles = static_cast<long long>((OC + n - 1) / n) * ((M + 255) / 256), pairs = sms / 2;
+  return 5.5 + static_cast<double>((tiles + pairs - 1) / pairs) * (static_cast<double>(steps) * step + 0.4);
+}
 // Channels of a pair's tile, or 0: the streaming form.
 int pair_columns(const glowq_w8a8_linear_t& g, int sms) {
-  if (const char* v = std::getenv("W8_TILE")) return std::atoi(v);
-  if (g.M <= 128) return 0;
+  if (g.M <= 64) return 0;
+  const bool corrected = g.r_mode != GLOWQ_R_NONE;
   // (a converted tile is held as sums / alpha: a factor near nothing would leave the range of fp32)
-  if (g.r_mode != GLOWQ_R_NONE && !(std::fabs(g.alpha) >= 0x1p-60f && std::fabs(g.alpha) <= 0x1p60f)) return 0;
-  const int n_y = (g.M + 255) / 256, pairs = sms / 2;
-  int best = 256;
-  long long best_cost = 0;
-  for (int n = 256; n >= 64; n -= 64) {
-    const long long tiles = static_cast<long long>((g.OC + n - 1) / n) * n_y, cost = (tiles + pairs - 1) / pairs * (2 * n + 60);
-    if (n == 256 || cost < best_cost) {
+  if (corrected && !(std::fabs(g.alpha) >= 0x1p-60f && std::fabs(g.alpha) <= 0x1p60f)) return 0;
+  const long long steps = (g.K + 127) / 128 + (corrected ? (g.rank + 63) / 64 : 0);
+  int best = 0;
+  double least = stream_us(g.M, steps, g.OC, sms);
+  for (int n = 64; n <= 256; n += 64) {
+    const double us = pair_us(g.M, steps, g.OC, n, sms);
+    if (us < least) {
       best = n;
-      best_cost = cost;
+      least = us;
     }
   }
   return best;
@@ -162,7 +180,7 @@ int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
       r.dtype = g.x_dtype;
       if ((rc = note_cuda_error(launch_rows(r, sms, stream))) != GLOWQ_OK) return rc;
     }
-    if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, true, sms, stream)) != GLOWQ_OK) return rc;
+    if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, g.x != nullptr, sms, stream)) != GLOWQ_OK) return rc;
   }
   const int n = pair_columns(g, sms);
   return n > 0 ? w8a8_pair_forward(g, n, sms, stream) : w8a8_stream_forward(g, sms, stream);

@@ -31,9 +31,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) few_tokens_ker
   const int t = threadIdx.x, step = blockDim.x * V, K = p.rows.K, M = p.rows.M;
   const auto column = [&](int i) { return min(t * V + i * step, K - V); };
   const __half* const x0 = static_cast<const __half*>(p.rows.x);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < M) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int row = blockIdx.x;
     Vec h[kNV];
     uint32_t top = 0u;
@@ -59,6 +59,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) few_tokens_ker
   for (int i = 0; i < kNV; ++i)
     unpack2<__half>(t * V + i * step < K ? ld16(p.R + j * p.R_stride + t * V + i * step) : Vec{}, w[i]);   // (zeros past the end)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Vec x[kFewTokens][kNV];
 #pragma unroll
   for (int m = 0; m < kFewTokens; ++m)

@@ -509,7 +509,6 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
   constexpr bool WARP = THREADS == 32;
   __shared__ double2 s_sum[3][32];
   __shared__ uint32_t s_max[2][32];
-  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, step = (WARP ? 32 : blockDim.x) * V, K = p.K;
   const int row0 = WARP ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x, rows = WARP ? gridDim.x * kWarpRows : gridDim.x;
   const T *const w = static_cast<const T*>(p.weight), *const b = static_cast<const T*>(p.bias);
@@ -530,6 +529,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
     }
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (only now: the launch behind may take it that all in front of this one is complete)
+  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (row0 < p.M) fetch(row0);
   int buf = 0;
   constexpr bool kAhead = THREADS > 256 && NV == kNV && MODE == kWhole;   // CTAs take row after row; else a row each
@@ -639,8 +640,8 @@ template <typename T, int NORM, bool CODES>
 __global__ void __launch_bounds__(kRowThreads) long_rows_kernel(const __grid_constant__ RowsParams p) {
   __shared__ double2 s_sum[32];
   __shared__ uint32_t s_max[32];
-  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int row = blockIdx.x, K = p.K;
   const T* const x = static_cast<const T*>(p.x) + row * p.xs;
   const T* const res = p.residual ? static_cast<const T*>(p.residual) + row * p.rs : nullptr;
@@ -774,10 +775,10 @@ template <typename T, int MODE, int NV, int ROWS, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_constant__ GradParams p) {
   constexpr int V = Num<T>::kVec;
   extern __shared__ float s_all[];                // [2][warps][2 ROWS], at the end [groups][2][K]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int g = threadIdx.x / p.group, t = threadIdx.x - g * p.group, groups = blockDim.x / p.group, step = p.group * V, K = p.K;
   const int nw = p.group >> 5, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // A group's rows lie `units` apart, a multiple of eight: all of them begin at the same place within 16 bytes.
   const int units = gridDim.x * groups, unit = blockIdx.x * groups + g, stride = units * ROWS;
   const int off = MODE == kSame ? row_offset(static_cast<const T*>(p.h) + unit * p.hs) : 0;
@@ -939,8 +940,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
 // dweight and dbias: the CTAs' parts, added in their order.
 template <typename T> __global__ void __launch_bounds__(256) norm_grad_sum_kernel(const __grid_constant__ GradParams p) {
   __shared__ float s_sum[8][32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const long long col = static_cast<long long>(blockIdx.x) * 32 + lane, cols = 2ll * p.K;   // dweight's columns, then dbias's
   float s = 0.f;
@@ -962,8 +963,8 @@ template <typename T> __global__ void __launch_bounds__(256) norm_grad_sum_kerne
 // Rows that do not fit a CTA: the sums over the columns first, then dx and the column sums of 256 columns x a share of the rows.
 template <typename T> __global__ void __launch_bounds__(kRowThreads) long_grad_sums_kernel(const __grid_constant__ GradParams p) {
   __shared__ double2 s_sum[32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int row = blockIdx.x;
   const T *const h = static_cast<const T*>(p.h) + row * p.hs, *const dy = static_cast<const T*>(p.dy) + row * p.ys;
   const float mean = p.mean[row], rstd = p.rstd[row];
@@ -981,8 +982,8 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) long_grad_s
   }
 }
 template <typename T> __global__ void __launch_bounds__(256) long_grad_kernel(const __grid_constant__ GradParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long k = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (k >= p.K) return;
   const float w = Num<T>::up(static_cast<const T*>(p.weight)[k]);

@@ -32,7 +32,7 @@ constexpr int kThreads = 224;
 // Dynamic shared memory at most: of a launch whose CTAs have an SM each, and of one that has more of them, two to an SM.
 constexpr int kSmemOne = 220 * 1024, kSmemTwo = 113 * 1024;
 constexpr int kMaxStages = 12;
-constexpr int kMaxSplit = 8;
+constexpr int kMaxSplit = 16;          // CTAs of a cluster (above 8 for r alone)
 constexpr unsigned kDrainSpin = 1u << 18;
 
 struct StreamParams {
@@ -42,6 +42,7 @@ struct StreamParams {
   int M, OC, out_dtype, vec;     // vec: four outputs are stored together
   int nk, nr, split;             // steps of the product and of the correction; CTAs of a cluster
   int early;                     // the launch behind this one may begin at once
+  int beside;                    // this launch may run beside the one in front, and ends after it
   float alpha;
 };
 struct alignas(64) StreamMaps {
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, TWO ? 2 : 1) stream_kernel(const __g
   };
   if (threadIdx.x == 0)
     for (int i = 0; i < ahead; ++i) load_a(it0 + i, smem0 + kFull + 8 * i, ring + i * kStage);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
   // (a constant: with a number of columns that the launch chose, an SM held one CTA instead of two)
   constexpr uint32_t columns = F16 ? (N < 32 ? 32 : N) : 2 * N;
   if (warp == 1) {
@@ -325,30 +326,38 @@ __global__ void __launch_bounds__(kThreads, TWO ? 2 : 1) stream_kernel(const __g
     store4(p, m0 + t, n0 + col, y);
   }
   if (split > 1) cluster_sync_all();   // the others' reads of this CTA's sums
+  if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // CTAs of a cluster: as many as leave all tiles in one round with an SM for each CTA (clusters of some sizes fill the SMs less well), each
 // with two steps at least.  us, one token, 5120 -> 5120 (40 tiles) in clusters of 1, 2, 3, 4: 10.1, 8.4, 7.4, 11.8; 77 tokens,
 // 18944 -> 3584 (28 tiles) in 1 to 5: 37.5, 23.3, 19.3, 17.2, 28.9.
-int plan_split(long long tiles, int steps, int sms) {
-  constexpr int kHeld[kMaxSplit + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};   // CTAs in clusters of 1 to 8 on 148 SMs
+int plan_split(long long tiles, int steps, int sms, int most) {
+  constexpr int kHeld[kMaxSplit + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120, 0, 0, 0, 0, 0, 0, 0, 112};   // CTAs in clusters of so many on 148 SMs
   int best = 1;
-  for (int s = 2; s <= std::min(kMaxSplit, steps / 2); ++s)
+  for (int s = 2; s <= std::min(most, steps / 2); ++s)
     if (tiles * s <= static_cast<long long>(kHeld[s]) * sms / 148) best = s;
   return best;
 }
+
+// (sixteen, of an SM each, where r's rows are long: 77 tokens, 18944 columns, rank 128: 13.0 us in eight, 9.7; 7 tokens, 5120: 5.5, so 6.1)
+int most_split(bool f16, int steps) { return f16 && steps >= 160 ? kMaxSplit : 8; }
 
 template <int N, bool F16, bool TWO>
 int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t stream) {
   constexpr int smem = smem_of<N, TWO>();
   const int x = (p.OC + kRows - 1) / kRows, y = (p.M + N - 1) / N;
-  p.split = TWO ? 1 : plan_split(static_cast<long long>(x) * y, p.nk + p.nr, sms);
+  p.split = TWO ? 1 : plan_split(static_cast<long long>(x) * y, p.nk + p.nr, sms, most_split(F16, p.nk));
   static bool attr_done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(stream_kernel<N, F16, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return note_cuda_error(e);
+    if (F16) {   // clusters of more than eight
+      const cudaError_t c = cudaFuncSetAttribute(stream_kernel<N, F16, TWO>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (c != cudaSuccess) return note_cuda_error(c);
+    }
     attr_done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -393,6 +402,8 @@ template <bool F16> int launch_tokens(const StreamParams& p, const StreamMaps& t
 
 cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream) { return take_status(g_w8a8_status, out, stream); }
 
+int w8a8_stream_split(long long tiles, int steps, int sms) { return plan_split(tiles, steps, sms, 8); }
+
 int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stream) {
   const bool corrected = g.r_mode != GLOWQ_R_NONE;
   const int n = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
@@ -420,8 +431,21 @@ int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stre
   return rc ? rc : launch_tokens<false>(p, tm, n, sms, stream);
 }
 
-int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool early, int sms, cudaStream_t stream) {
-  const int n = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
+int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, int sms, cudaStream_t stream) {
+  // Tokens of a tile: those with which a CTA reads least (narrow tiles read R once more each, but there are more CTAs).  77 tokens, 18944
+  // columns, rank 128: one tile of 128 tokens in 8 CTAs 13.0 us, five of 16 in 16 each 9.7.
+  int n = 128;
+  double least = 0.0;
+  for (int t = 16; t <= 128; t *= 2) {
+    const long long tiles = static_cast<long long>((g.rank + kRows - 1) / kRows) * ((g.M + t - 1) / t);
+    const int steps = (g.K + 63) / 64, split = plan_split(tiles, steps, sms, most_split(true, steps));
+    const double rounds = static_cast<double>((tiles * split + sms - 1) / sms);
+    const double cost = rounds * ((steps + split - 1) / split) * (kAStage + t * 128);
+    if (t == 16 || cost < least) {
+      n = t;
+      least = cost;
+    }
+  }
   StreamParams p{};
   p.out = g.r;
   p.out_stride = g.r_stride;
@@ -430,7 +454,7 @@ int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool early, int sms, cudaStr
   p.OC = g.rank;
   p.nk = (g.K + 63) / 64;
   p.vec = g.r_stride % 4 == 0;
-  p.early = early;
+  p.early = p.beside = beside;   // (in front of the product, behind the codes of the same x)
   StreamMaps tm;
   int rc = tensor_map_2d_ex(&tm.a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.R, g.K, g.rank, 2 * g.R_stride, 64, kRows, 1);
   if (!rc) rc = tensor_map_2d_ex(&tm.b, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.r_x, g.K, g.M, 2 * g.r_x_stride, 64, n, 1);

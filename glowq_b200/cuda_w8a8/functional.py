@@ -209,7 +209,10 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     """One 8-bit linear.  ``x``: activations [..., in_features] (their codes are made here), or ``TokenCodes`` -> [tokens, out_features].
     ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
     [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, fp16 for codes.  ``L`` fp16 [out_features, rank]:
-    the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``."""
+    the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``.
+
+    ``weight``, ``L`` and ``R`` may be read before the launch in front of this one is complete: they are constants, not results of this
+    package's calls right in front (except ``quantize_channels``)."""
     x2 = lead = r = None
     if isinstance(x, TokenCodes):
         codes, scales, r = x

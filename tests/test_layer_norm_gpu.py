@@ -128,7 +128,9 @@ def test_some_gradients_only():
     y, h = w8.layer_norm(t[0], t[1], t[2], EPS, t[3])
     g = torch.autograd.grad(h, t, dy, retain_graph=True)
     assert torch.equal(g[0], dy) and torch.equal(g[3], dy) and not g[1].any() and not g[2].any()
-    g = torch.autograd.grad(y, t, dy)
+    g = torch.autograd.grad(y, t, dy, retain_graph=True)
+    (y * dy).sum().backward()
+    assert t[0].grad.data_ptr() != t[3].grad.data_ptr() and torch.equal(t[0].grad, t[3].grad)
     assert_within(g[0], *exact((x.double() + res.double()).float(), w, b, dy)[1])
     # without a bias
     t = [u.clone().requires_grad_() for u in (x, w)]

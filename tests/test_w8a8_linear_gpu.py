@@ -212,6 +212,17 @@ def test_weights_made_right_before_they_are_used():
         del q, qs
 
 
+@pytest.mark.parametrize("m,k,n", [(260, 256, 2000), (260, 256, 4000), (260, 256, 5000), (260, 256, 9000), (600, 384, 20000), (1500, 130, 9000),
+                                   (70, 640, 30000), (40, 256, 20001)])
+def test_tiles_of_every_width_and_rounds_of_them(m, k, n):
+    """Pairs on tiles of 64 to 256 channels, one and several to a pair (a corrected tile ends among the next one's steps), two CTAs to an SM."""
+    x, q, qs, b, L, R = operands(m, k, n, 72)
+    t = w8.quantize_tokens(x)._replace(r=w8.right_factor(x, R))
+    for out in (torch.float16, torch.float32):
+        assert_within(w8.w8a8_linear(t, q, qs, b, out_dtype=out), *product_of(*codes_of(x), q, qs, b))
+        assert_within(w8.w8a8_linear(t, q, qs, b, out_dtype=out, L=L, alpha=0.6), *product_of(*codes_of(x), q, qs, b, 0.6, t.r, L))
+
+
 def test_many_channels_and_tokens():
     for m, k, n in ((5000, 128, 300), (9, 128, 40_000), (1, 64, 70_001)):
         x, q, qs, b = operands(m, k, n)
