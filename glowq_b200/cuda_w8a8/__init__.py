@@ -6,7 +6,7 @@ correction, if there is one), and the norms in front of them.  The reference pro
     q, k, v = q_proj(tokens), k_proj(tokens), v_proj(tokens)           # CudaW8A8Linear modules
 """
 from .functional import (TokenCodes, norm_quantize_tokens, quantize_channels, quantize_tokens, read_status, right_factor, w8a8_linear)
-from .layer_norm import CudaLayerNorm, layer_norm
+from .norms import CudaLayerNorm, layer_norm
 from .linear import CudaW8A8Linear, convert_to_cuda_w8a8
 
 __all__ = ["TokenCodes", "quantize_tokens", "norm_quantize_tokens", "quantize_channels", "right_factor", "w8a8_linear", "layer_norm",

@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 
 from .functional import TokenCodes, _pitch, quantize_channels, quantize_tokens, right_factor, w8a8_linear
-from .layer_norm import CudaLayerNorm
+from .norms import CudaLayerNorm
 
 
 class CudaW8A8Linear(nn.Module):
@@ -20,6 +20,16 @@ class CudaW8A8Linear(nn.Module):
         self.register_buffer("qweight_i8", torch.zeros(self.out_features, _pitch(self.in_features), dtype=torch.int8))
         self.register_buffer("scales_f32", torch.zeros(self.out_features, dtype=torch.float32))
         self.bias = nn.Parameter(torch.zeros(self.out_features, dtype=torch.float32), requires_grad=False) if bias else None
+
+    def _apply(self, fn, recurse: bool = True):
+        """Moves with the model; scales and bias stay fp32 whatever type the model is cast to."""
+        scales, bias = self.scales_f32, self.bias.data if self.bias is not None else None   # (a parameter is cast in place)
+        super()._apply(fn, recurse)
+        if self.scales_f32.dtype != torch.float32:
+            self.scales_f32 = scales.to(self.scales_f32.device)
+        if bias is not None and self.bias.dtype != torch.float32:
+            self.bias.data = bias.to(self.bias.device)
+        return self
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

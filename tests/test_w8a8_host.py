@@ -65,6 +65,17 @@ def test_module_and_conversion():
         w8.CudaLayerNorm((2, 3))
 
 
+def test_modules_that_are_cast():
+    """A model cast to another type: codes, scales and bias stay what they are."""
+    mod = w8.CudaW8A8Linear.from_float(nn.Linear(24, 16))
+    want = {k: v.clone() for k, v in mod.state_dict().items()}
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu")):
+        model = cast(nn.Sequential(mod))
+        for k, v in mod.state_dict().items():
+            assert v.dtype == want[k].dtype and torch.equal(v, want[k])
+        assert isinstance(model[0].bias, nn.Parameter)
+
+
 def test_cpu_tensors_are_refused():
     x, w = torch.randn(2, 16), torch.ones(16)
     for call in (lambda: w8.quantize_tokens(x), lambda: w8.norm_quantize_tokens(x, w), lambda: w8.layer_norm(x, w),

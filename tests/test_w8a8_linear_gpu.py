@@ -194,6 +194,32 @@ def test_graphs_and_streams(m):
     w8.read_status()
 
 
+def test_threads():
+    """Calls from several threads at once, each on a stream of its own."""
+    import threading
+    jobs = []
+    for i, m in enumerate((1, 3, 60, 300)):
+        x, q, qs, b, L, R = operands(m, 1024, 512, 64, seed=i)
+        jobs.append((x, q, qs, b, L, R, w8.w8a8_linear(x, q, qs, b, L=L, R=R)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, q, qs, b, L, R, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                y = w8.w8a8_linear(x, q, qs, b, L=L, R=R)
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(y, want):
+                wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_weights_made_right_before_they_are_used():
     """Weights that the call in front quantised: the product does not read them early."""
     gen = torch.Generator(device="cuda").manual_seed(0)
