@@ -92,11 +92,15 @@ def quantize_tokens(x: torch.Tensor) -> TokenCodes:
     """int8 codes and a scale for every row of ``x`` [..., in_features] (fp16, bf16 or fp32), in one launch."""
     x = _rows(x, "x")
     (m, k), dev = x.shape, x.device
-    codes = _new_codes(m, k, dev)
+    pitch = (k + 15) & ~15
+    codes = _empty(m, pitch, dtype=_int8, device=dev)
     scales = _empty(m, dtype=_float32, device=dev)
     if m:
-        _quantize(x, codes, scales, False)
-    return TokenCodes(codes, scales)
+        # (_quantize, without the calls)
+        desc = _pack_rows(x.data_ptr(), 0, 0, 0, 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0, current_stream_ptr(dev), 0.0, x.stride()[0],
+                          0, 0, 0, pitch, m, k, K.DTYPES[x.dtype], 0, 0, 0)
+        K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
+    return TokenCodes(codes if pitch == k else codes[:, :k], scales)
 
 
 def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -165,12 +169,11 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
 
 def check_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
     """(``x``: what ``_rows`` gave)"""
-    k, dtype, dev = x.shape[1], x.dtype, x.device
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None and name == "bias":
-            continue
-        if t is None or t.dtype != dtype or t.device != dev or t.dim() != 1 or t.shape[0] != k:
-            raise RuntimeError(f"{name} must be [{k}] of x's type on x's device")
+    shape, dtype, dev = (x.shape[1],), x.dtype, x.device
+    if weight is None or weight.shape != shape or weight.dtype != dtype or weight.device != dev:
+        raise RuntimeError(f"weight must be [{shape[0]}] of x's type on x's device")
+    if bias is not None and (bias.shape != shape or bias.dtype != dtype or bias.device != dev):
+        raise RuntimeError(f"bias must be [{shape[0]}] of x's type on x's device")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
 
@@ -219,7 +222,7 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         if not codes.is_cuda or codes.dtype != _int8 or codes.dim() != 2:
             raise RuntimeError("codes must be int8 [tokens, in_features] on a CUDA device")
         (m, k), dev = codes.shape, codes.device
-        if scales.dtype != _float32 or scales.dim() != 1 or scales.shape[0] != m or scales.device != dev:
+        if scales.dtype != _float32 or scales.shape != (m,) or scales.device != dev:
             raise RuntimeError(f"scales must be fp32 [{m}] on {dev}")
         if R is not None:
             raise RuntimeError("codes have no right factor's product to be made from: pass TokenCodes.r (right_factor(x, R))")
@@ -244,9 +247,10 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         raise ValueError(f"Input dim mismatch: got {k}, expected {ic}")
     if not 0 < k <= K.MAX_EXACT_K:
         raise RuntimeError(f"in_features must be 1 to {K.MAX_EXACT_K} (sums are exact in 32 bits)")
-    for t, name in ((weight_scales, "weight_scales"), (bias, "bias")):
-        if t is not None and (t.dtype != _float32 or t.dim() != 1 or t.shape[0] != oc or t.device != dev):
-            raise RuntimeError(f"{name} must be fp32 [{oc}] on {dev}")
+    if weight_scales.dtype != _float32 or weight_scales.shape != (oc,) or weight_scales.device != dev:
+        raise RuntimeError(f"weight_scales must be fp32 [{oc}] on {dev}")
+    if bias is not None and (bias.dtype != _float32 or bias.shape != (oc,) or bias.device != dev):
+        raise RuntimeError(f"bias must be fp32 [{oc}] on {dev}")
     if m > K.MAX_TOKENS:
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
     out = _empty(m, oc, dtype=out_dtype, device=dev)
