@@ -767,7 +767,9 @@ template <typename T> cudaError_t launch_rows_typed(const RowsParams& p, int nor
 // ---------------------------------------------------------------- gradients of the layer norm
 // A CTA holds one or several groups of threads that have a row's columns between them (NV pieces of 16 bytes a thread); a group takes ROWS
 // rows at a time, and the next ones' loads go out before these are worked on.  A thread keeps to its columns: the sums of dweight and
-// dbias stay in its registers until the end.  Reads h, dy (dh) and writes dx once: bound by memory.
+// dbias stay in its registers until the end.  Reads h, dy (dh) and writes dx once.  32768 x 2048 fp16 87 us (floor 61.6), 8192 x 5120 bf16
+// 79 (38.5): bound by issue slots, 23 instructions an element, a third of them moves and addresses, and by a barrier for every round.
+// (A warp along each row first and threads down its columns then, the second reads from L1: 26 instructions, 117 us.)
 constexpr int kGradParts = 304;    // CTAs of the gradients at most, whatever the device: their number fixes the order of the sums
 constexpr int kGradThreads = 1024;
 

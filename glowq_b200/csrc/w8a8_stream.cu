@@ -12,6 +12,8 @@
 // at work whatever the number of channels; their sums meet in shared memory (each CTA reads its share of the others' blocks),
 // integers in any order, the correction's fp32 sums in the order of the CTAs: no workspace, no counters, the same bits every time.
 //   warps 0 and 6  copies (a thread each)    warp 1  tensor memory, MMAs    warps 2-5  sums to shared memory; all: scales, bias, output
+//   One token, 2048 -> 2048 4.5 us, 5120 -> 5120 6.8 (3.9 TB/s), 5120 -> 13824 13.1 (5.4); 16 tokens, 5120 -> 27648 25.2 (5.6); 77 tokens,
+// 18944 -> 3584 14.1 (4.9): a chain of some 4 us - launch, first weights, a cluster's sum - and the copy rate.
 // Tensor memory is taken after the dependency wait: a CTA that held it while it waits could keep a kernel in front from taking its own.
 #include <cuda_bf16.h>
 
