@@ -271,3 +271,38 @@ def test_how_far_eight_bits_are():
     s = codes_of(x)[1].double()
     limit = 0.5 * s[:, None] * w.abs().sum(dim=1)            # the tokens' rounding; the weights are their codes here
     assert ((y.double() - x.double() @ w.t()).abs() <= limit * (1 + 1e-5) + HALF_STEP[torch.float32]).all()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows' codes, norms, products and r."""
+    m, k, n = 131_104, 16_400, 72
+    if torch.cuda.get_device_properties(0).total_memory < 40e9:
+        pytest.skip("needs 40 GB")
+    x = torch.zeros(m, k, dtype=torch.float16, device="cuda")
+    rows = torch.tensor([0, 5, m // 2, m - 200, m - 1], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    some = torch.randn(len(rows), k, generator=gen, device="cuda").half()
+    x[rows] = some
+    t = w8.quantize_tokens(x)
+    codes, scales = codes_of(some)
+    assert torch.equal(t.codes[rows], codes) and torch.equal(t.scales[rows], scales)
+    _, q, qs, b, L, R = operands(1, k, n, 24)
+    r = w8.right_factor(x, R)
+    assert_within(r[rows], *right_factor_of(some, R))
+    y = w8.w8a8_linear(t._replace(r=r), q, qs, b, L=L, alpha=0.5)
+    want, bound = product_of(codes, scales, q, qs, b, 0.5, r[rows], L)
+    assert_within(y[rows], want, bound)
+    assert_within(y[1:5], *product_of(torch.zeros_like(codes[:4]), torch.zeros_like(scales[:4]), q, qs, b, 0.5, r[1:5], L))
+    del t, y
+    w = torch.ones(k, dtype=torch.float16, device="cuda")
+    ln = w8.layer_norm(x, w)
+    assert torch.equal(ln[rows], w8.layer_norm(some, w)) and not ln[1].any()
+    del ln
+    leaf, wl = x.requires_grad_(), w.clone().requires_grad_()
+    dy = torch.zeros(m, k, dtype=torch.float16, device="cuda")
+    dy[rows] = some.flip(0)
+    gx, gw = torch.autograd.grad(w8.layer_norm(leaf, wl), (leaf, wl), dy)
+    small = some.clone().requires_grad_()
+    sx, _ = torch.autograd.grad(w8.layer_norm(small, wl), (small, wl), some.flip(0))
+    # (row sums in the same order whatever the number of rows)
+    assert torch.equal(gx[rows], sx) and not gx[1].any()
