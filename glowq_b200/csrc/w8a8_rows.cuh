@@ -1023,7 +1023,8 @@ GradPlan grad_plan(int M, int K, int vec, bool same) {
   g.rows = g.nv && g.group * g.groups <= 256 ? 2 : 1;
   const int per = g.rows * g.groups;
   g.parts = std::max(1, std::min(g.nv && g.group <= 512 ? 296 : 148, g.nv ? (M + per - 1) / per : M / 16));
-  if (same) g.parts = (g.parts + 7) / 8 * 8;   // (then the rows of a group lie a multiple of eight apart)
+  // (the rows of a group lie a multiple of eight apart, and no CTA is left for a second round)
+  if (same && g.nv) g.parts = std::max(8, g.parts / 8 * 8);
   const int warps = g.group * g.groups / 32;
   g.smem = std::max<size_t>(2ull * warps * 2 * g.rows, g.groups > 1 ? 2ull * g.groups * K : 0) * 4;
   return g;
