@@ -4,13 +4,17 @@
 //
 // All of it is bound by memory: a row is read once, stays in registers through the norm, the maximum and the codes, and every output is
 // written once.  A row belongs to a CTA of as many threads as it has pieces of 4 x 16 bytes (to one warp up to 1024 16-bit columns,
-// several rows to a CTA then); CTAs take row after row, and a row's loads go out before the row in front of it is worked on, so that the
-// SM's loads never stop.  Values stay in their own type in registers (16 for 32 16-bit values), which leaves room for that.
-//   Rows that do not begin on 16 bytes are read in 16-byte pieces all the same, two per piece of the row, shifted together; they are
-// written so too, with what the lane in front holds.  (Element by element 4097 x 4999 fp16 took 39 us, floor 9.4.)
+// several rows to a CTA then).  Values stay in their own type in registers (16 for 32 16-bit values), so that an SM holds 1024 threads'
+// rows; above 256 threads a row, CTAs take row after row, and a row's loads go out before the row in front of it is worked on.
+//   Rows that do not begin on 16 bytes are read in 16-byte pieces all the same (see Mode).  (Element by element 4097 x 4999 fp16 took
+// 39 us, floor 9.4; so 16.)
 //   A code is the nearest integer of the EXACT quotient, ties to even: it does not hang on how a division rounds.  Products with a little
-// less and a little more than 1 / s have the same nearest integer but where a border is near (one value in some ten thousand); there the
-// remainder v - n s, which one FMA gives exactly, decides.
+// less and a little more than 1 / s have the same nearest integer but where a border is near (one value in some ten thousand; of 8-bit
+// mantissas, many of whose quotients are halves, one in some hundred); there the side of the border that v is on decides, which one FMA
+// gives exactly.
+//   us (floor): codes of 4096 x 13824 fp16 28.2 (26.0), bf16 32.8, fp32 44.3 (43.3); residual + RMSNorm + codes of 4000 x 5120 fp16 25.5
+// (21.9), with a layer norm 28.6; layer norm of 32768 x 2048 fp16 47.6 (41.1).  What is left is bound by issue slots: 11 to 25 instructions
+// an element.
 //   The statistics of a norm are sums in 64 bits, rounded to fp32 once, so that they - and with them every code - do not depend on the
 // order of the sums.  var = S2/K - (S1/K)^2 from one pass over the registers; where the difference costs more than 20 of the 53 bits (rows
 // whose mean is a thousand times their deviation) a second pass sums the squares around the mean.
@@ -501,7 +505,7 @@ template <int NORM> __device__ __forceinline__ Stats make_stats(double mean, dou
   return Stats{NORM == GLOWQ_NORM_LAYER ? static_cast<float>(mean) : 0.f, static_cast<float>(rsqrt(var + eps))};
 }
 
-// Rows by a CTA of up to THREADS threads, or (THREADS = 32) by a warp; so many CTAs to an SM that a thread has 64 to 85 registers.
+// Rows by a CTA of up to THREADS threads, or (THREADS = 32) by a warp; so many CTAs to an SM that a thread has 64 registers.
 constexpr int row_ctas(int threads) { return threads == 32 ? 8 : threads == 256 ? 4 : threads == 512 ? 2 : 1; }
 template <typename T, int NORM, bool RES, bool CODES, int MODE, int THREADS, int NV = kNV>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_ctas(THREADS)) rows_kernel(const __grid_constant__ RowsParams p) {
