@@ -817,19 +817,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
   int buf = 0;
   for (int base = blockIdx.x * groups; base < p.M; base += stride, buf ^= 1) {   // (the same number of rounds for all groups)
     const int r0 = base + g;
-    // xh = h rstd - mean rstd, and dy; zeros past the end of a row (dy) and past the last row (dy)
+    // xh = (h - mean) rstd, as the forward pass has it (h rstd - mean rstd in one FMA rounds mean rstd: a constant row of 999 would give
+    // dweight 0.006 dy), and dy; zeros past the end of a row (dy) and past the last row (dy)
     F2 xh[ROWS][NV][V / 2], d[ROWS][NV][V / 2];
     float rstd[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       rstd[r] = nrstd[r];
-      const F2 rs2 = pair_of(rstd[r], rstd[r]), shift = pair_of(-nmean[r] * rstd[r], -nmean[r] * rstd[r]);
+      const F2 rs2 = pair_of(rstd[r], rstd[r]), shift = pair_of(-nmean[r], -nmean[r]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         unpack2<T>(nh[r][i], xh[r][i]);
         unpack2<T>(nd[r][i], d[r][i]);
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) xh[r][i][j] = fma2(xh[r][i][j], rs2, shift);
+        for (int j = 0; j < V / 2; ++j) xh[r][i][j] = mul2(add2(xh[r][i][j], shift), rs2);
       }
     }
     if (base + stride < p.M) fetch(r0 + stride);

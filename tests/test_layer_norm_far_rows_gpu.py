@@ -1,0 +1,70 @@
+"""Layer norm's gradients on rows that lie far from zero against their deviation: the row's mean is taken off first, whatever its size."""
+import pytest
+import torch
+
+from glowq_b200 import cuda_w8a8 as w8
+from w8a8_reference import U, assert_within
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+EPS = 1e-5
+# (of each plan: a group of warps, a CTA to a row, two pieces a thread, passes over the rows; odd widths)
+WIDTHS = [64, 250, 1000, 2048, 2999, 5120, 9000, 12288, 40000]
+
+
+def gradients(h, w, dy):
+    """(dx, bound), (dw, bound), (db, bound) in 64 bits of rows whose mean is a number of 32 bits."""
+    v, m = h.double(), h.shape[0]
+    total = v.sum(dim=1, keepdim=True)                    # (exact: 24 bits and the count's)
+    mean = total / torch.full_like(total, h.shape[1])     # (a scalar divisor would be taken as a product with its reciprocal)
+    assert torch.equal(mean, mean.float().double())
+    rstd = 1 / torch.sqrt((v - mean).square().mean(dim=1, keepdim=True) + EPS)
+    xh = (v - mean) * rstd
+    exh = 4 * U * xh.abs()                    # a difference, rstd, a product: the mean is exact
+    d, g = dy.double(), dy.double() * w.double()
+    c1, c2 = g.mean(dim=1, keepdim=True), (g * xh).mean(dim=1, keepdim=True)
+    n = 140 * U                               # sums over a row: at most 128 additions in a thread, then a tree of 10
+    ec1, ec2 = n * g.abs().mean(dim=1, keepdim=True), n * (g * xh).abs().mean(dim=1, keepdim=True) + (g.abs() * exh).mean(dim=1, keepdim=True)
+    dx = rstd * (g - c1 - xh * c2)
+    edx = rstd * (6 * U * (g.abs() + c1.abs() + (xh * c2).abs()) + ec1 + xh.abs() * ec2 + exh * (c2.abs() + ec2))
+    rows = (m + 12) * U
+    return ((dx, edx * 1.01), ((d * xh).sum(dim=0), 1.01 * (rows * (d * xh).abs().sum(dim=0) + (d.abs() * exh).sum(dim=0))),
+            (d.sum(dim=0), 1.01 * rows * d.abs().sum(dim=0)))
+
+
+def leaves(m, k, dtype, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    return (1 + 0.3 * rand(k)).to(dtype).requires_grad_(), rand(k).to(dtype).requires_grad_(), rand(m, k).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", WIDTHS)
+def test_constant_rows(k, dtype):
+    """What is normalised is zero: dweight gets nothing from such rows."""
+    for value in (999.0, -0.7, 3.0e4):
+        w, b, dy = leaves(9, k, dtype)
+        x = torch.full((9, k), value, device="cuda").to(dtype).requires_grad_()
+        gx, gw, gb = torch.autograd.grad(w8.layer_norm(x, w, b, EPS), (x, w, b), dy)
+        assert not gw.any()
+        dx, _, db = gradients(x.detach(), w.detach(), dy)
+        assert_within(gx, *dx, "dx")
+        assert_within(gb, *db, "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", WIDTHS)
+def test_rows_with_a_large_mean(k, dtype):
+    """16384 +- a few steps of the type, in equal parts: the mean is exact, and some hundred deviations."""
+    m, step = 21, {torch.float16: 16, torch.bfloat16: 128, torch.float32: 16}[dtype]
+    w, b, dy = leaves(m, k, dtype, seed=k)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.full((m, k), 16384.0, device="cuda")
+    for row in range(m):
+        signs = 2 * (torch.randperm(k // 2 * 2, generator=gen, device="cuda") % 2) - 1
+        x[row, k % 2:] += step * (3 + 2 * (row % 3)) * signs
+    x = x.to(dtype)
+    want = gradients(x, w.detach(), dy)
+    x.requires_grad_()
+    for got, (value, bound), name in zip(torch.autograd.grad(w8.layer_norm(x, w, b, EPS), (x, w, b), dy), want, ("dx", "dw", "db")):
+        assert_within(got, value, bound, name)
