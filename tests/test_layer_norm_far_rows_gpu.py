@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from glowq_b200 import cuda_w8a8 as w8
-from w8a8_reference import U, assert_within
+from w8a8_reference import U, assert_within, codes_of, norm_of
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
@@ -68,3 +68,23 @@ def test_rows_with_a_large_mean(k, dtype):
     x.requires_grad_()
     for got, (value, bound), name in zip(torch.autograd.grad(w8.layer_norm(x, w, b, EPS), (x, w, b), dy), want, ("dx", "dw", "db")):
         assert_within(got, value, bound, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [37, 96, 1001, 2999, 5121, 5128, 9001, 12290, 40001])
+def test_rows_of_the_lowest_value(k, dtype):
+    """Rows that a mask has filled with the type's lowest value (mean * rstd is above all numbers): what lies behind a row's end joins no sum."""
+    lowest = torch.finfo(dtype).min
+    w, b, dy = leaves(9, k, dtype, seed=k)
+    x = torch.randn(9, k, device="cuda").to(dtype)
+    x[::2] = lowest
+    for res in (None, torch.zeros_like(x)):
+        t, h = w8.norm_quantize_tokens(x, w.detach(), b.detach(), eps=EPS, residual=res, norm="layer")
+        _, y, _, _ = norm_of(x, None, w.detach(), b.detach(), EPS, "layer")
+        codes, scales = codes_of(y)
+        assert torch.equal(h, x) and torch.equal(t.scales, scales) and torch.equal(t.codes, codes)
+        assert torch.equal(y[0], b)
+    leaf = x[::2].clone().requires_grad_()
+    gx, gw, gb = torch.autograd.grad(w8.layer_norm(leaf, w, b, EPS), (leaf, w, b), dy[::2].contiguous())
+    assert not gw.any() and torch.isfinite(gx).all()
+    assert_within(gb, *gradients(leaf.detach(), w.detach(), dy[::2])[2], "db")
