@@ -583,12 +583,14 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
       const double mean = sum.x * p.inv_k;
       double var = sum.y * p.inv_k - mean * mean;
       if (NORM == GLOWQ_NORM_LAYER && var < 0x1p-20 * mean * mean) {
-        // more than 20 bits went in the difference: once more, around the mean (and from memory, which takes no registers from the others)
+        // more than 20 bits went in the difference: once more, around the mean (and from memory, which takes no registers from the others;
+        // a quotient, which is exact where the mean is: a constant row's deviation is nothing, not 2^-53 of its value)
+        const double mu = sum.x / K;
         double2 s = make_double2(0.0, 0.0);
         const T *const xr = x_row(row), *const rr = RES ? r_row(row) : nullptr;
         for (int k = t; k < K; k += step / V) {
           const float f = RES ? rounded<T>(Num<T>::up(xr[k]) + Num<T>::up(rr[k])) : Num<T>::up(xr[k]);
-          const double d = static_cast<double>(f) - mean;
+          const double d = static_cast<double>(f) - mu;
           s.y = fma(d, d, s.y);
         }
         var = row_sum<WARP, false>(s, s_sum[2]).y * p.inv_k;
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_kernel(const __grid_con
     double mean = 0.0;
     if (NORM == GLOWQ_NORM_LAYER) {
       for (int k = threadIdx.x; k < K; k += blockDim.x) sum.x += value(k);
-      mean = row_sum<false, true>(sum, s_sum).x * p.inv_k;
+      mean = row_sum<false, true>(sum, s_sum).x / K;
       __syncthreads();
     }
     for (int k = threadIdx.x; k < K; k += blockDim.x) {

@@ -88,3 +88,17 @@ def test_rows_of_the_lowest_value(k, dtype):
     gx, gw, gb = torch.autograd.grad(w8.layer_norm(leaf, w, b, EPS), (leaf, w, b), dy[::2].contiguous())
     assert not gw.any() and torch.isfinite(gx).all()
     assert_within(gb, *gradients(leaf.detach(), w.detach(), dy[::2])[2], "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [37, 96, 1001, 2999, 5121, 5128, 9001, 12290, 40001])
+def test_deviation_of_constant_rows(k, dtype):
+    """It is nothing at any width, however large the value: dx is the projection of dy * weight, times 1 / sqrt(eps)."""
+    w, b, dy = leaves(3, k, dtype, seed=k)
+    for value in (torch.finfo(dtype).min, min(1e20, torch.finfo(dtype).max)):
+        x = torch.full((3, k), value, dtype=dtype, device="cuda", requires_grad=True)
+        gx, gw, gb = torch.autograd.grad(w8.layer_norm(x, w, b, EPS), (x, w, b), dy)
+        dx, _, db = gradients(x.detach(), w.detach(), dy)
+        assert_within(gx, *dx, "dx")
+        assert_within(gb, *db, "db")
+        assert not gw.any()
