@@ -10,7 +10,10 @@ namespace {
 
 constexpr int kMaxExactK = 131071;     // 128 * 128 * K stays below 2^31: the sums of products are exact
 constexpr int kMaxRank = 1024;
-constexpr int kMaxTokens = 1 << 22;    // tiles of 64 tokens are numbered by 16 bits of a grid
+constexpr int kMaxTokens = 1 << 22;    // tiles of 128 tokens (above 64 there are no narrower ones) are numbered by 16 bits of a grid
+// Rows and columns of the kernels that count them in 32 bits: a row and all rows, a column and a CTA's columns, both halves of the
+// gradients' sums stay below 2^31.
+constexpr int kMaxRows = 1 << 30, kMaxColumns = 1 << 29;
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool known(int dtype) { return dtype == GLOWQ_F16 || dtype == GLOWQ_F32 || dtype == GLOWQ_BF16; }
@@ -25,6 +28,7 @@ int check_rows(const glowq_w8a8_rows_t& r, bool codes) {
   if (r.norm == GLOWQ_NORM_NONE ? r.weight || r.residual || r.mean || r.rstd : !r.weight || !(r.eps >= 0.0)) return GLOWQ_ERR_BAD_ARGUMENT;
   if ((r.bias && r.norm != GLOWQ_NORM_LAYER) || (r.hidden && !r.residual) || (r.constant && r.norm != GLOWQ_NORM_NONE))
     return GLOWQ_ERR_BAD_ARGUMENT;
+  if (r.M > kMaxRows || r.K > kMaxColumns) return GLOWQ_ERR_TOO_LARGE;
   if (r.M == 0) return GLOWQ_OK;
   if (!r.x || (codes ? !r.codes || !r.scales : !r.y)) return GLOWQ_ERR_BAD_ARGUMENT;
   const size_t e = dtype_bytes(r.dtype);
@@ -54,7 +58,7 @@ int check_operand(const void* p, int64_t stride, size_t e, int rows, int cols) {
 
 int check_right_factor(const glowq_w8a8_linear_t& g) {
   if (g.M < 0 || g.K <= 0 || g.rank <= 0 || g.reserved != 0) return GLOWQ_ERR_BAD_ARGUMENT;
-  if (g.M > kMaxTokens || g.rank > kMaxRank) return GLOWQ_ERR_TOO_LARGE;
+  if (g.M > kMaxTokens || g.K > kMaxColumns || g.rank > kMaxRank) return GLOWQ_ERR_TOO_LARGE;
   if (g.M == 0) return GLOWQ_OK;
   int rc = check_operand(g.r_x, g.r_x_stride, 2, g.M, g.K);
   if (!rc) rc = check_operand(g.R, g.R_stride, 2, g.rank, g.K);
@@ -65,7 +69,7 @@ int check_right_factor(const glowq_w8a8_linear_t& g) {
 int check_linear(const glowq_w8a8_linear_t& g) {
   if (g.M < 0 || g.K <= 0 || g.OC <= 0 || g.rank < 0 || g.reserved != 0 || !known(g.out_dtype)) return GLOWQ_ERR_BAD_ARGUMENT;
   if (g.r_mode != GLOWQ_R_NONE && g.r_mode != GLOWQ_R_COMPUTE && g.r_mode != GLOWQ_R_LOAD) return GLOWQ_ERR_BAD_ARGUMENT;
-  if (g.K > kMaxExactK || g.M > kMaxTokens) return GLOWQ_ERR_TOO_LARGE;
+  if (g.K > kMaxExactK || g.M > kMaxTokens || g.OC > kMaxColumns) return GLOWQ_ERR_TOO_LARGE;
   if (g.M == 0) return GLOWQ_OK;
   if (!g.scales || !g.weight_scales || !g.out || !aligned(g.out, dtype_bytes(g.out_dtype)) || !aligned(g.scales, 4) ||
       !aligned(g.weight_scales, 4) || !aligned(g.bias, 4))
@@ -135,6 +139,7 @@ int glowq_layer_norm_backward(const glowq_layer_norm_grad_t* grad) {
   if (g.M <= 0 || g.K <= 0 || g.reserved != 0 || !known(g.dtype)) return GLOWQ_ERR_BAD_ARGUMENT;
   if (!g.h || !g.dy || !g.weight || !g.mean || !g.rstd || (!g.dweight) != (!g.dbias) || (!g.dx && !g.dweight) || (g.dh && !g.dx))
     return GLOWQ_ERR_BAD_ARGUMENT;
+  if (g.M > kMaxRows || g.K > kMaxColumns) return GLOWQ_ERR_TOO_LARGE;
   const size_t e = dtype_bytes(g.dtype);
   for (const void* p : {g.h, g.dy, g.dh, g.weight, static_cast<const void*>(g.dx), static_cast<const void*>(g.dweight),
                         static_cast<const void*>(g.dbias)})

@@ -439,11 +439,12 @@ int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, int sms, cudaSt
   int n = 128;
   double least = 0.0;
   for (int t = 16; t <= 128; t *= 2) {
+    if (g.M > 65535 * t) continue;   // (a grid's second dimension)
     const long long tiles = static_cast<long long>((g.rank + kRows - 1) / kRows) * ((g.M + t - 1) / t);
     const int steps = (g.K + 63) / 64, split = plan_split(tiles, steps, sms, most_split(true, steps));
     const double rounds = static_cast<double>((tiles * split + sms - 1) / sms);
     const double cost = rounds * ((steps + split - 1) / split) * (kAStage + t * 128);
-    if (t == 16 || cost < least) {
+    if (least == 0.0 || cost < least) {
       n = t;
       least = cost;
     }

@@ -32,7 +32,7 @@ enum { GLOWQ_NORM_NONE = 0, GLOWQ_NORM_LAYER = 1, GLOWQ_NORM_RMS = 2 };
  *     scale = fp32(max |v| / 127),  code = the integer nearest to v / scale, ties to even, exactly, within [-127, 127]
  * "round" is to the matrix's own type.  A row of zeros has scale 0 and codes 0.  A row with a NaN or an infinity has scale NaN and
  * codes 0, so that every output of that token is NaN.  Strides are in elements; rows have unit column stride; no output overlaps an
- * input or another output. */
+ * input or another output.  At most 2^30 rows and 2^29 columns, here and in the layer norm's gradients. */
 typedef struct glowq_w8a8_rows {
   const void* x;          /* [M, x_stride]                                                       */
   const void* residual;   /* [M, residual_stride] or NULL                                        */
@@ -85,7 +85,8 @@ int glowq_layer_norm_backward(const glowq_layer_norm_grad_t* grad);
 /* One linear.  With `x` set the call first quantises x into `codes` and `scales` (which are then scratch of the caller's); with r_mode
  * GLOWQ_R_COMPUTE it computes r = r_x . R^T (rounded to fp16, as the W4A16 path holds it) into `r`; GLOWQ_R_LOAD takes r as it is.
  * Alignment: codes, weight, r_x, R, L and r begin on 16 bytes and their row strides are multiples of 16 bytes (what lies behind
- * column K is never used); out and bias need the alignment of their elements.  K <= 131071 (exact sums); rank <= 1024.
+ * column K is never used); out and bias need the alignment of their elements.  K <= 131071 (exact sums); rank <= 1024; at most 2^22
+ * tokens and 2^29 channels.
  * `weight`, `weight_scales`, `bias`, L and R may be read before the calls in front of this one on the stream are complete, if those are
  * calls of this library: they must not be results of such calls, except of glowq_w8a8_quantize with `constant`. */
 typedef struct glowq_w8a8_linear {
