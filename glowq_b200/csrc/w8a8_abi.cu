@@ -45,7 +45,10 @@ int run_rows(const glowq_w8a8_rows_t* rows, bool codes) {
   int rc = check_rows(*rows, codes), sms = 0;
   if (rc == GLOWQ_OK) rc = current_device_sms(&sms);
   if (rc != GLOWQ_OK || rows->M == 0) return rc;
-  return note_cuda_error(launch_rows(*rows, sms, static_cast<cudaStream_t>(rows->stream)));
+  const cudaStream_t stream = static_cast<cudaStream_t>(rows->stream);
+  cudaError_t e = launch_rows(*rows, sms, stream);
+  if (e == cudaSuccess && rows->constant) e = launch_settle(stream);
+  return note_cuda_error(e);
 }
 
 // operands that the copy engine reads: they begin on 16 bytes, and so does every row
@@ -159,19 +162,23 @@ int glowq_w8a8_right_factor(const glowq_w8a8_linear_t* linear) {
   int rc = check_right_factor(*linear), sms = 0;
   if (rc == GLOWQ_OK) rc = current_device_sms(&sms);
   if (rc != GLOWQ_OK || linear->M == 0) return rc;
-  return w8a8_right_factor(*linear, false, sms, static_cast<cudaStream_t>(linear->stream));
+  return w8a8_right_factor(*linear, false, (linear->r_mode & GLOWQ_W8A8_FRESH) == 0, sms, static_cast<cudaStream_t>(linear->stream));
 }
 
 int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
   if (!linear) return GLOWQ_ERR_BAD_ARGUMENT;
   glowq_w8a8_linear_t g = *linear;
+  // Operands that were made right in front: the call's first launch waits for that as any kernel does.  (Codes' launch reads none of them,
+  // and those behind it begin when it is past its own wait.)
+  const bool ahead = (g.r_mode & GLOWQ_W8A8_FRESH) == 0;
+  g.r_mode &= ~GLOWQ_W8A8_FRESH;
   int rc = check_linear(g), sms = 0;
   if (rc == GLOWQ_OK) rc = current_device_sms(&sms);
   if (rc != GLOWQ_OK || g.M == 0) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(g.stream);
   if (g.alpha == 0.f) g.r_mode = GLOWQ_R_NONE;   // nothing to add
   if (g.x && g.r_mode == GLOWQ_R_COMPUTE && few_tokens(g)) {
-    if ((rc = note_cuda_error(launch_few_tokens(g, stream))) != GLOWQ_OK) return rc;
+    if ((rc = note_cuda_error(launch_few_tokens(g, ahead, stream))) != GLOWQ_OK) return rc;
   } else {
     if (g.x) {
       glowq_w8a8_rows_t r{};
@@ -185,10 +192,12 @@ int glowq_w8a8_linear(const glowq_w8a8_linear_t* linear) {
       r.dtype = g.x_dtype;
       if ((rc = note_cuda_error(launch_rows(r, sms, stream))) != GLOWQ_OK) return rc;
     }
-    if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, g.x != nullptr, sms, stream)) != GLOWQ_OK) return rc;
+    if (g.r_mode == GLOWQ_R_COMPUTE && (rc = w8a8_right_factor(g, g.x != nullptr, ahead || g.x, sms, stream)) != GLOWQ_OK) return rc;
   }
   const int n = pair_columns(g, sms);
-  return n > 0 ? w8a8_pair_forward(g, n, sms, stream) : w8a8_stream_forward(g, sms, stream);
+  // (behind another launch of this call, that one was waited for)
+  const bool first = !g.x && g.r_mode != GLOWQ_R_COMPUTE;
+  return n > 0 ? w8a8_pair_forward(g, n, ahead || !first, sms, stream) : w8a8_stream_forward(g, ahead || !first, sms, stream);
 }
 
 int glowq_w8a8_read_status(void* stream) {

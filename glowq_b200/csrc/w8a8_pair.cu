@@ -436,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 cudaError_t w8a8_pair_status(uint32_t* out, cudaStream_t stream) { return take_status(g_w8a8_pair_status, out, stream); }
 
-int w8a8_pair_forward(const glowq_w8a8_linear_t& g, int n, int sms, cudaStream_t stream) {
+int w8a8_pair_forward(const glowq_w8a8_linear_t& g, int n, bool ahead, int sms, cudaStream_t stream) {
   const bool corrected = g.r_mode != GLOWQ_R_NONE;
   PairParams p{};
   p.scales = g.scales;
@@ -493,7 +493,7 @@ int w8a8_pair_forward(const glowq_w8a8_linear_t& g, int n, int sms, cudaStream_t
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = use_pdl() ? 1 : 0;
+  cfg.numAttrs = ahead && use_pdl() ? 1 : 0;
   return note_cuda_error(cudaLaunchKernelEx(&cfg, w8a8_pair_kernel, p, tm));
 }
 

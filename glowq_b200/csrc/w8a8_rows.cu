@@ -96,7 +96,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) few_tokens_ker
 
 cudaError_t launch_rows(const glowq_w8a8_rows_t& r, int sms, cudaStream_t stream) {
   const RowsParams p{r.x,        r.residual,        r.weight,        r.bias,     r.hidden,      r.y, r.codes, r.scales, r.mean, r.rstd, r.eps, 1.0 / r.K,
-                     r.x_stride, r.residual_stride, r.hidden_stride, r.y_stride, r.code_stride, r.M, r.K,     r.constant};
+                     r.x_stride, r.residual_stride, r.hidden_stride, r.y_stride, r.code_stride, r.M, r.K};
   if (r.dtype == GLOWQ_F16) return launch_rows_f16(p, r.norm, sms, stream);
   if (r.dtype == GLOWQ_BF16) return launch_rows_bf16(p, r.norm, sms, stream);
   return launch_rows_f32(p, r.norm, sms, stream);
@@ -107,7 +107,7 @@ bool few_tokens(const glowq_w8a8_linear_t& g) {
   return g.M <= kFewTokens && g.x == g.r_x && g.x_dtype == GLOWQ_F16 && (g.M == 1 || g.x_stride == g.r_x_stride) && g.K % 8 == 0 &&
          g.K <= 8 * kNV * kRowThreads && whole(g.x, g.M > 1 ? g.x_stride : 0);
 }
-cudaError_t launch_few_tokens(const glowq_w8a8_linear_t& g, cudaStream_t stream) {
+cudaError_t launch_few_tokens(const glowq_w8a8_linear_t& g, bool ahead, cudaStream_t stream) {
   FewParams p{};
   p.rows.x = g.x;
   p.rows.xs = g.x_stride;
@@ -121,8 +121,16 @@ cudaError_t launch_few_tokens(const glowq_w8a8_linear_t& g, cudaStream_t stream)
   p.r = static_cast<__half*>(g.r);
   p.r_stride = g.r_stride;
   const int threads = ((g.K / 8 + kNV - 1) / kNV + 31) / 32 * 32;
-  if (threads <= 256) return launch(few_tokens_kernel<256>, dim3(g.M + g.rank), threads, stream, p);
-  return launch(few_tokens_kernel<kRowThreads>, dim3(g.M + g.rank), threads, stream, p);
+  if (threads <= 256) return launch(few_tokens_kernel<256>, dim3(g.M + g.rank), threads, stream, p, ahead);
+  return launch(few_tokens_kernel<kRowThreads>, dim3(g.M + g.rank), threads, stream, p, ahead);
+}
+
+__global__ void settle_kernel() {}
+cudaError_t launch_settle(cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = cfg.blockDim = dim3(1);
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, settle_kernel);
 }
 
 size_t layer_norm_grad_bytes(int M, int K) {

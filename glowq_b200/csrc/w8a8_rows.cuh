@@ -36,7 +36,7 @@ struct RowsParams {
   float *scales, *mean, *rstd;
   double eps, inv_k;
   long long xs, rs, hs, ys, cs;
-  int M, K, constant;
+  int M, K;
 };
 struct GradParams {
   const void *h, *dy, *dh, *weight;
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // (only now: the launch behind may take it that all in front of this one is complete)
-  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (row0 < p.M) fetch(row0);
   int buf = 0;
   constexpr bool kAhead = THREADS > 256 && NV == kNV && MODE == kWhole;   // CTAs take row after row; else a row each
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_kernel(const __grid_con
   __shared__ double2 s_sum[32];
   __shared__ uint32_t s_max[32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!p.constant) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int row = blockIdx.x, K = p.K;
   const T* const x = static_cast<const T*>(p.x) + row * p.xs;
   const T* const res = p.residual ? static_cast<const T*>(p.residual) + row * p.rs : nullptr;
@@ -712,8 +712,9 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_kernel(const __grid_con
   }
 }
 
+// ahead: the kernel may begin while the one in front of it still runs (it waits for its end by itself)
 template <typename Kernel, typename Params>
-cudaError_t launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const Params& p) {
+cudaError_t launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const Params& p, bool ahead = true) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -722,7 +723,7 @@ cudaError_t launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = use_pdl() ? 1 : 0;
+  cfg.numAttrs = ahead && use_pdl() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

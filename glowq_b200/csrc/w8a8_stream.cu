@@ -346,7 +346,7 @@ int plan_split(long long tiles, int steps, int sms, int most) {
 int most_split(bool f16, int steps) { return f16 && steps >= 160 ? kMaxSplit : 8; }
 
 template <int N, bool F16, bool TWO>
-int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t stream) {
+int launch_stream(StreamParams p, const StreamMaps& tm, bool ahead, int sms, cudaStream_t stream) {
   constexpr int smem = smem_of<N, TWO>();
   const int x = (p.OC + kRows - 1) / kRows, y = (p.M + N - 1) / N;
   p.split = TWO ? 1 : plan_split(static_cast<long long>(x) * y, p.nk + p.nr, sms, most_split(F16, p.nk));
@@ -369,7 +369,7 @@ int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t st
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (use_pdl()) {
+  if (ahead && use_pdl()) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
@@ -383,21 +383,21 @@ int launch_stream(StreamParams p, const StreamMaps& tm, int sms, cudaStream_t st
   cfg.numAttrs = n;
   return note_cuda_error(cudaLaunchKernelEx(&cfg, stream_kernel<N, F16, TWO>, p, tm));
 }
-template <int N, bool F16> int launch_ring(const StreamParams& p, const StreamMaps& tm, int sms, cudaStream_t stream) {
+template <int N, bool F16> int launch_ring(const StreamParams& p, const StreamMaps& tm, bool ahead, int sms, cudaStream_t stream) {
   static_assert((F16 ? 1 : 2) * N * kRows * 4 <= smem_of<N, false>() - 2048, "the sums fit the ring");
   // Two CTAs to an SM where one each would leave a second round: 16 tokens, 5120 -> 27648 (216 tiles) 25.5 us, so 29.3; with one round
   // the deeper ring: 5120 -> 13824 (108 tiles) 13.1 us, so 14.7.  (Their rings do not hold the two blocks of sums of 128 tokens.)
   if constexpr (N <= 64) {
     static_assert((F16 ? 1 : 2) * N * kRows * 4 <= smem_of<N, true>() - 2048, "the sums fit the ring");
-    if (static_cast<long long>((p.OC + kRows - 1) / kRows) * ((p.M + N - 1) / N) > sms) return launch_stream<N, F16, true>(p, tm, sms, stream);
+    if (static_cast<long long>((p.OC + kRows - 1) / kRows) * ((p.M + N - 1) / N) > sms) return launch_stream<N, F16, true>(p, tm, ahead, sms, stream);
   }
-  return launch_stream<N, F16, false>(p, tm, sms, stream);
+  return launch_stream<N, F16, false>(p, tm, ahead, sms, stream);
 }
-template <bool F16> int launch_tokens(const StreamParams& p, const StreamMaps& tm, int n, int sms, cudaStream_t stream) {
-  if (n == 16) return launch_ring<16, F16>(p, tm, sms, stream);
-  if (n == 32) return launch_ring<32, F16>(p, tm, sms, stream);
-  if (n == 64) return launch_ring<64, F16>(p, tm, sms, stream);
-  return launch_ring<128, F16>(p, tm, sms, stream);
+template <bool F16> int launch_tokens(const StreamParams& p, const StreamMaps& tm, int n, bool ahead, int sms, cudaStream_t stream) {
+  if (n == 16) return launch_ring<16, F16>(p, tm, ahead, sms, stream);
+  if (n == 32) return launch_ring<32, F16>(p, tm, ahead, sms, stream);
+  if (n == 64) return launch_ring<64, F16>(p, tm, ahead, sms, stream);
+  return launch_ring<128, F16>(p, tm, ahead, sms, stream);
 }
 
 }  // namespace
@@ -406,7 +406,7 @@ cudaError_t w8a8_stream_status(uint32_t* out, cudaStream_t stream) { return take
 
 int w8a8_stream_split(long long tiles, int steps, int sms) { return plan_split(tiles, steps, sms, 8); }
 
-int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stream) {
+int w8a8_stream_forward(const glowq_w8a8_linear_t& g, bool ahead, int sms, cudaStream_t stream) {
   const bool corrected = g.r_mode != GLOWQ_R_NONE;
   const int n = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   StreamParams p{};
@@ -430,10 +430,10 @@ int w8a8_stream_forward(const glowq_w8a8_linear_t& g, int sms, cudaStream_t stre
     rc = tensor_map_2d_ex(&tm.l, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.L, g.rank, g.OC, 2 * g.L_stride, 64, kRows, 1);
     if (!rc) rc = tensor_map_2d_ex(&tm.r, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.r, g.rank, g.M, 2 * g.r_stride, 64, n, 1);
   }
-  return rc ? rc : launch_tokens<false>(p, tm, n, sms, stream);
+  return rc ? rc : launch_tokens<false>(p, tm, n, ahead, sms, stream);
 }
 
-int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, int sms, cudaStream_t stream) {
+int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, bool ahead, int sms, cudaStream_t stream) {
   // Tokens of a tile: those with which a CTA reads least (narrow tiles read R once more each, but there are more CTAs).  77 tokens, 18944
   // columns, rank 128: one tile of 128 tokens in 8 CTAs 13.0 us, five of 16 in 16 each 9.7.
   int n = 128;
@@ -461,7 +461,7 @@ int w8a8_right_factor(const glowq_w8a8_linear_t& g, bool beside, int sms, cudaSt
   StreamMaps tm;
   int rc = tensor_map_2d_ex(&tm.a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.R, g.K, g.rank, 2 * g.R_stride, 64, kRows, 1);
   if (!rc) rc = tensor_map_2d_ex(&tm.b, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.r_x, g.K, g.M, 2 * g.r_x_stride, 64, n, 1);
-  return rc ? rc : launch_tokens<true>(p, tm, n, sms, stream);
+  return rc ? rc : launch_tokens<true>(p, tm, n, ahead, sms, stream);
 }
 
 }  // namespace glowq

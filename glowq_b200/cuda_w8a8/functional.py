@@ -65,21 +65,22 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def _place(t: torch.Tensor, e: int):
-    """(tensor, address, row stride) of a matrix of ``e``-byte elements as the copy engine reads it: rows that begin on 16 bytes.  (Others
-    are copied; what the package makes lies so.  Of a single row the stride may be anything: the library is told one that it accepts.)"""
+    """(tensor, address, row stride, flag) of a matrix of ``e``-byte elements as the copy engine reads it: rows that begin on 16 bytes.
+    (Others are copied; what the package makes lies so.  Of a single row the stride may be anything: the library is told one that it
+    accepts.)  The flag is ``K.FRESH`` for a copy, which a launch right behind it may not read early, else 0."""
     at, (rows, cols), (s0, s1) = t.data_ptr(), t.shape, t.stride()
     if not at & 15 and s1 == 1:
         if rows > 1:
             if s0 >= cols and not s0 * e & 15:
-                return t, at, s0
+                return t, at, s0, 0
         else:
             per = 16 // e
-            return t, at, (cols + per - 1) // per * per
+            return t, at, (cols + per - 1) // per * per, 0
     per = 16 // e
     pitch = (cols + per - 1) // per * per
     room = _empty(rows, pitch, dtype=t.dtype, device=t.device)
     room[:, :cols].copy_(t)
-    return room, room.data_ptr(), pitch
+    return room, room.data_ptr(), pitch, K.FRESH
 
 
 def _quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, constant: bool) -> None:
@@ -185,37 +186,39 @@ def _factor(t: torch.Tensor, name: str, rows: int, cols: Optional[int], device):
     return _place(t.detach() if t.requires_grad else t, 2)
 
 
-def right_factor(x: torch.Tensor, R: torch.Tensor) -> torch.Tensor:
+def right_factor(x: torch.Tensor, R: torch.Tensor, constant: bool = True) -> torch.Tensor:
     """r = x R^T, fp16 [tokens, rank], for corrected linears that share a right factor (``TokenCodes.r``).  ``x`` is taken in fp16, as the
-    W4A16 path takes it; sums in fp32."""
+    W4A16 path takes it; sums in fp32.  ``constant``: as for ``w8a8_linear``."""
     x = _rows(x.detach(), "x")
     if R.dim() != 2 or not 0 < R.shape[0] <= K.MAX_RANK:
         raise RuntimeError(f"R must be [rank, in_features] with a rank of 1 to {K.MAX_RANK}")
     (m, k), dev = x.shape, x.device
     if m > K.MAX_TOKENS:
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
-    R, R_at, R_stride = _factor(R, "R", R.shape[0], k, dev)
+    R, R_at, R_stride, fresh = _factor(R, "R", R.shape[0], k, dev)
     rank = R.shape[0]
+    if not constant:
+        fresh = K.FRESH
     pitch = (rank + 7) & ~7
     r = _empty(m, pitch, dtype=_float16, device=dev)
     if m:
-        x, x_at, x_stride = _place(x if x.dtype == _float16 else x.to(_float16), 2)
+        x, x_at, x_stride, _ = _place(x if x.dtype == _float16 else x.to(_float16), 2)
         desc = _pack_linear(0, 0, 0, 0, 0, 0, x_at, R_at, r.data_ptr(), 0, 0, current_stream_ptr(dev), 0, 0, 0, x_stride, R_stride, pitch, 0,
-                            0, m, k, 0, rank, 0, 0, K.R_COMPUTE, 0.0, 0)
+                            0, m, k, 0, rank, 0, 0, K.R_COMPUTE | fresh, 0.0, 0)
         K.call(K.ext().right_factor, dev, desc, "glowq_w8a8_right_factor")
     return r if pitch == rank else r[:, :rank]
 
 
 def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight_scales: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, *, out_dtype: Optional[torch.dtype] = None, L: Optional[torch.Tensor] = None,
-                R: Optional[torch.Tensor] = None, alpha: float = 1.0) -> torch.Tensor:
+                R: Optional[torch.Tensor] = None, alpha: float = 1.0, constant: bool = True) -> torch.Tensor:
     """One 8-bit linear.  ``x``: activations [..., in_features] (their codes are made here), or ``TokenCodes`` -> [tokens, out_features].
     ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
     [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, fp16 for codes.  ``L`` fp16 [out_features, rank]:
     the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``.
 
-    ``weight``, ``L`` and ``R`` may be read before the launch in front of this one is complete: they are constants, not results of this
-    package's calls right in front (except ``quantize_channels``)."""
+    ``constant``: ``weight``, ``L`` and ``R`` may be read before what is in front of this call on the stream is complete.  Pass False where
+    the operation right in front made one of them (a merge, a cast, a copy; what ``quantize_channels`` gives may be used at once)."""
     x2 = lead = r = None
     if isinstance(x, TokenCodes):
         codes, scales, r = x
@@ -255,7 +258,9 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
     out = _empty(m, oc, dtype=out_dtype, device=dev)
     if m and oc:
-        weight, w_at, w_stride = _place(weight, 1)
+        weight, w_at, w_stride, fresh = _place(weight, 1)
+        if not constant:
+            fresh = K.FRESH
         weight_scales = weight_scales.contiguous()
         b_at = 0
         if bias is not None:
@@ -264,20 +269,22 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = x_at = x_stride = x_code = 0
         if L is not None:
             rank = L.shape[1] if L.dim() == 2 else 0
-            L, L_at, L_stride = _factor(L, "L", oc, None, dev)
+            L, L_at, L_stride, copied = _factor(L, "L", oc, None, dev)
+            fresh |= copied
             if not 0 < rank <= K.MAX_RANK:
                 raise RuntimeError(f"the rank must be 1 to {K.MAX_RANK}")
             if x2 is None:
                 if r is None:
                     raise RuntimeError("a corrected linear of codes needs TokenCodes.r (right_factor(x, R))")
-                r, r_at, r_stride = _factor(r, "r", m, rank, dev)
+                r, r_at, r_stride, _ = _factor(r, "r", m, rank, dev)
                 mode = K.R_LOAD
             else:
-                R, R_at, R_stride = _factor(R, "R", rank, k, dev)
-                rx, rx_at, rx_stride = _place((x2 if x2.dtype == _float16 else x2.to(_float16)).detach(), 2)
+                R, R_at, R_stride, copied = _factor(R, "R", rank, k, dev)
+                fresh |= copied
+                rx, rx_at, rx_stride, _ = _place((x2 if x2.dtype == _float16 else x2.to(_float16)).detach(), 2)
                 mode = K.R_COMPUTE
         if x2 is None:
-            codes, code_at, code_stride = _place(codes, 1)
+            codes, code_at, code_stride, _ = _place(codes, 1)
             scales = scales.contiguous()
             scale_at = scales.data_ptr()
         else:
@@ -291,7 +298,7 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
             scale_at, r_at = code_at + scale_off, code_at + r_off
         desc = _pack_linear(x_at, code_at, scale_at, w_at, weight_scales.data_ptr(), b_at, rx_at, R_at, r_at, L_at, out.data_ptr(),
                             current_stream_ptr(dev), x_stride, code_stride, w_stride, rx_stride, R_stride, r_stride, L_stride, oc, m, k, oc,
-                            rank, x_code, out_code, mode, alpha, 0)
+                            rank, x_code, out_code, mode | fresh, alpha, 0)
         K.call(K.ext().linear, dev, desc, "glowq_w8a8_linear")
     return out if lead is None else out.reshape(*lead, oc)
 

@@ -10,7 +10,7 @@ from ..cuda_w4a16 import kernels as K
 
 F16, F32, BF16 = 0, 1, 2
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
-R_NONE, R_COMPUTE, R_LOAD = K.R_NONE, K.R_COMPUTE, K.R_LOAD
+R_NONE, R_COMPUTE, R_LOAD, FRESH = K.R_NONE, K.R_COMPUTE, K.R_LOAD, 16
 MAX_EXACT_K, MAX_RANK, MAX_TOKENS = 131071, 1024, 1 << 22
 DTYPES = {torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16}
 

@@ -50,7 +50,7 @@ typedef struct glowq_w8a8_rows {
   int32_t M, K;
   int32_t dtype;          /* GLOWQ_F16 / GLOWQ_F32 / GLOWQ_BF16: x, residual, weight, bias, hidden, y */
   int32_t norm;           /* GLOWQ_NORM_*                                                        */
-  int32_t constant;       /* nonzero: the codes are weights - a product launched behind this call may not read them early */
+  int32_t constant;       /* nonzero: the codes are weights, which a product launched behind this call may read early */
   int32_t reserved;       /* must be 0                                                           */
 } glowq_w8a8_rows_t;
 
@@ -82,13 +82,17 @@ typedef struct glowq_layer_norm_grad {
 size_t glowq_layer_norm_workspace_bytes(int M, int K);
 int glowq_layer_norm_backward(const glowq_layer_norm_grad_t* grad);
 
+/* Added to r_mode below. */
+enum { GLOWQ_W8A8_FRESH = 16 };
+
 /* One linear.  With `x` set the call first quantises x into `codes` and `scales` (which are then scratch of the caller's); with r_mode
  * GLOWQ_R_COMPUTE it computes r = r_x . R^T (rounded to fp16, as the W4A16 path holds it) into `r`; GLOWQ_R_LOAD takes r as it is.
  * Alignment: codes, weight, r_x, R, L and r begin on 16 bytes and their row strides are multiples of 16 bytes (what lies behind
  * column K is never used); out and bias need the alignment of their elements.  K <= 131071 (exact sums); rank <= 1024; at most 2^22
  * tokens and 2^29 channels.
- * `weight`, `weight_scales`, `bias`, L and R may be read before the calls in front of this one on the stream are complete, if those are
- * calls of this library: they must not be results of such calls, except of glowq_w8a8_quantize with `constant`. */
+ * `weight`, `weight_scales`, `bias`, L and R are constants: they may be read before what is in front of this call on the stream is complete
+ * and visible, whoever launched it.  Where the kernel, copy or call right in front made one of them, add GLOWQ_W8A8_FRESH to r_mode
+ * (glowq_w8a8_quantize with `constant` is complete for all that is launched behind it). */
 typedef struct glowq_w8a8_linear {
   const void* x;                /* [M, x_stride] of x_dtype, or NULL: codes and scales are there already */
   int8_t* codes;                /* [M, code_stride]                                                      */
