@@ -22,10 +22,12 @@ _pack_rows, _pack_linear = K.pack_rows.pack, K.pack_linear.pack
 
 class TokenCodes(NamedTuple):
     """A linear's input as int8 codes [tokens, in_features] with an fp32 scale per token [tokens].  ``r``: the right factor's product
-    with the same input, fp16 [tokens, rank], for corrected linears that share one.  Rows of codes lie a multiple of 16 bytes apart."""
+    with the same input, fp16 [tokens, rank], for corrected linears that share one.  ``dtype``: the input's type, which a linear's output
+    takes by default.  Rows of codes lie a multiple of 16 bytes apart."""
     codes: torch.Tensor
     scales: torch.Tensor
     r: Optional[torch.Tensor] = None
+    dtype: Optional[torch.dtype] = None
 
 
 # (Small calls cost what the host does: sizes in the place of a tuple and a known device take a third off an allocation, 0.8 us.)
@@ -101,7 +103,7 @@ def quantize_tokens(x: torch.Tensor) -> TokenCodes:
         desc = _pack_rows(x.data_ptr(), 0, 0, 0, 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0, current_stream_ptr(dev), 0.0, x.stride()[0],
                           0, 0, 0, pitch, m, k, K.DTYPES[x.dtype], 0, 0, 0)
         K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
-    return TokenCodes(codes if pitch == k else codes[:, :k], scales)
+    return TokenCodes(codes if pitch == k else codes[:, :k], scales, None, x.dtype)
 
 
 def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -165,7 +167,7 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
         K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
     if residual is not None and x.dim() != 2:
         hidden = hidden.reshape(x.shape)
-    return TokenCodes(codes, scales), hidden
+    return TokenCodes(codes, scales, None, x.dtype), hidden
 
 
 def check_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
@@ -214,14 +216,15 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
                 R: Optional[torch.Tensor] = None, alpha: float = 1.0, constant: bool = True) -> torch.Tensor:
     """One 8-bit linear.  ``x``: activations [..., in_features] (their codes are made here), or ``TokenCodes`` -> [tokens, out_features].
     ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
-    [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, fp16 for codes.  ``L`` fp16 [out_features, rank]:
+    [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, that which codes
+    were made of (fp16 where ``TokenCodes.dtype`` is None).  ``L`` fp16 [out_features, rank]:
     the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``.
 
     ``constant``: ``weight``, ``L`` and ``R`` may be read before what is in front of this call on the stream is complete.  Pass False where
     the operation right in front made one of them (a merge, a cast, a copy; what ``quantize_channels`` gives may be used at once)."""
     x2 = lead = r = None
     if isinstance(x, TokenCodes):
-        codes, scales, r = x
+        codes, scales, r, made_of = x
         if not codes.is_cuda or codes.dtype != _int8 or codes.dim() != 2:
             raise RuntimeError("codes must be int8 [tokens, in_features] on a CUDA device")
         (m, k), dev = codes.shape, codes.device
@@ -230,7 +233,7 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         if R is not None:
             raise RuntimeError("codes have no right factor's product to be made from: pass TokenCodes.r (right_factor(x, R))")
         if out_dtype is None:
-            out_dtype = _float16
+            out_dtype = made_of or _float16
     else:
         x2 = _rows(x, "x")
         (m, k), dev = x2.shape, x2.device
