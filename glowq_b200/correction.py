@@ -289,8 +289,8 @@ class AddSVDCorrection(nn.Module):
         if not isinstance(inner, (CudaW4A16Linear, CudaW8A8Linear)):
             raise TypeError("AddSVDCorrection wraps CudaW4A16Linear and CudaW8A8Linear modules only (no Triton / dense backends here)")
         self.inner = inner
-        self.register_buffer("A_q", A_q.to(torch.float16).contiguous(), persistent=False)
-        self.register_buffer("B_q", B_q.to(torch.float16).contiguous(), persistent=False)
+        self.register_buffer("A_q", self._laid(A_q.to(torch.float16)), persistent=False)
+        self.register_buffer("B_q", self._laid(B_q.to(torch.float16)), persistent=False)
         self.role = role
         self.is_group = is_group
         self.group_cache = group_cache
@@ -304,6 +304,29 @@ class AddSVDCorrection(nn.Module):
         if self._mismatch:
             warnings.warn(f"AddSVDCorrection: factor shapes A{tuple(A_q.shape)} B{tuple(B_q.shape)} do not fit "
                           f"linear {inner.in_features}->{inner.out_features}; correction disabled for this module")
+
+    def _laid(self, t: torch.Tensor) -> torch.Tensor:
+        """A factor as the inner linear reads it: dense, or for the 8-bit ones rows that begin on 16 bytes (a call copies others)."""
+        if isinstance(self.inner, CudaW4A16Linear) or t.dim() != 2 or (t.size(1) % 8 == 0 and t.is_contiguous()):
+            return t.contiguous()
+        if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.size(1):
+            return t
+        room = torch.zeros(t.size(0), (t.size(1) + 7) // 8 * 8, dtype=t.dtype, device=t.device)
+        room[:, :t.size(1)] = t
+        return room[:, :t.size(1)]
+
+    def _apply(self, fn, recurse: bool = True):
+        """Moves with the model; the factors stay fp16 whatever type it is cast to."""
+        held = {"A_q": self.A_q.detach(), "B_q": self.B_q.detach()}
+        super()._apply(fn, recurse)
+        for name, t in held.items():
+            now = getattr(self, name)
+            laid = self._laid(now.detach() if now.dtype == torch.float16 else t.to(now.device))
+            if isinstance(now, nn.Parameter):
+                now.data = laid
+            elif laid.dtype != now.dtype or laid.data_ptr() != now.data_ptr():
+                setattr(self, name, laid)
+        return self
 
     def _private_r(self, m: int, rank: int, device) -> torch.Tensor:
         if not isinstance(self._own_r, K.RRows):
