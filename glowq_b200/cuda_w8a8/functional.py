@@ -109,25 +109,32 @@ def quantize_tokens(x: torch.Tensor) -> TokenCodes:
 def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of a weight [out_features, in_features], a scale for every output channel.  The codes are a view of rows that lie a
     multiple of 16 bytes apart.  On the CPU the same codes with torch expressions, so that a model can be converted there."""
+    rows, scales = channel_rows(weight)
+    return rows[:, :weight.shape[1]], scales
+
+
+def channel_rows(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes in whole rows [out_features, in_features rounded up to 16] with zeros at the end, scales)"""
     if weight.dim() != 2 or weight.dtype not in K.DTYPES:
         raise RuntimeError("weight must be [out_features, in_features] in fp16, bf16 or fp32")
     weight = weight.detach()
     oc, ic = weight.shape
-    codes = torch.zeros((oc, _pitch(ic)), dtype=torch.int8, device=weight.device)[:, :ic]
+    rows = torch.zeros((oc, _pitch(ic)), dtype=torch.int8, device=weight.device)
+    codes = rows[:, :ic]
     scales = torch.empty(oc, dtype=torch.float32, device=weight.device)
     if oc == 0:
-        return codes, scales
+        return rows, scales
     if weight.is_cuda:
         weight = _rows(weight, "weight")
         _quantize(weight, codes, scales, True)
-        return codes, scales
+        return rows, scales
     top = weight.float().abs().amax(dim=1)
     torch.div(top, torch.full_like(top, 127.0), out=scales)
     bad = ~torch.isfinite(top)
     scales[bad] = float("nan")
     q = torch.round(weight.double() / scales.double()[:, None]).clamp_(-127, 127)
     codes.copy_(torch.where((scales > 0)[:, None], q, torch.zeros_like(q)))
-    return codes, scales
+    return rows, scales
 
 
 def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,

@@ -7,7 +7,7 @@ from typing import Optional, Union
 import torch
 import torch.nn as nn
 
-from .functional import TokenCodes, _pitch, quantize_channels, quantize_tokens, right_factor, w8a8_linear
+from .functional import TokenCodes, _pitch, channel_rows, quantize_tokens, right_factor, w8a8_linear
 from .norms import CudaLayerNorm
 
 
@@ -54,11 +54,10 @@ class CudaW8A8Linear(nn.Module):
     @classmethod
     def from_float(cls, linear_layer: nn.Linear, out_dtype: Optional[torch.dtype] = None) -> "CudaW8A8Linear":
         weight = linear_layer.weight.data
-        codes, scales = quantize_channels(weight)
+        rows, scales = channel_rows(weight)
         with torch.device("meta"):
             mod = cls(linear_layer.in_features, linear_layer.out_features, bias=linear_layer.bias is not None, out_dtype=out_dtype)
-        # (the rows as they were made: the view's base)
-        mod.qweight_i8 = codes._base if codes._base is not None else codes
+        mod.qweight_i8 = rows
         mod.scales_f32 = scales
         if linear_layer.bias is not None:
             mod.bias = nn.Parameter(linear_layer.bias.data.to(torch.float32).clone(), requires_grad=False)
