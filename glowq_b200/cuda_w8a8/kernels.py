@@ -81,10 +81,19 @@ def ext() -> _Ext:
 
 
 _device_now = K.current_device
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def _proxies() -> bool:
+    return torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
 
 
 def call(fn, device: torch.device, desc: bytes, what: str) -> None:
-    """``fn(desc)`` with ``device`` current."""
+    """``fn(desc)`` with ``device`` current.  Not under a trace of torch's operations, which does not see these calls and would keep
+    nothing but the allocation of their outputs."""
+    if _tracing() or (_modes() and _proxies()):
+        raise RuntimeError(f"{what} cannot be traced (torch.jit.trace, make_fx); capture a CUDA graph")
     if _device_now() == device.index:
         rc = fn(desc)
     else:
