@@ -18,6 +18,7 @@ from . import kernels as K
 
 _NORMS = {"layer": K.NORM_LAYER, "rms": K.NORM_RMS}
 _pack_rows, _pack_linear = K.pack_rows.pack, K.pack_linear.pack
+_TYPES = {code: dtype for dtype, code in K.DTYPES.items()}
 
 
 class TokenCodes(NamedTuple):
@@ -44,12 +45,21 @@ def _new_codes(m: int, k: int, device) -> torch.Tensor:
     return t if pitch == k else t[:, :k]
 
 
+def _matrix(x: torch.Tensor, name: str):
+    """``x`` as [rows, columns] with unit column stride and rows that do not overlap: (the matrix, rows, columns, row stride, device, the
+    library's code of the type).  What is asked of a tensor costs up to 0.1 us each time, so it is asked once."""
+    code = K.DTYPES.get(x.dtype)
+    if code is not None and x.is_cuda:      # (mostly all is well)
+        shape = x.shape
+        if len(shape) == 2:
+            (m, k), (s0, s1) = shape, x.stride()
+            if s1 == 1 and k > 0 and (s0 >= k or m <= 1):
+                return x, m, k, s0, x.device, code
+    x = _rows(x, name)
+    return x, x.shape[0], x.shape[1], x.stride()[0], x.device, K.DTYPES[x.dtype]
+
+
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """``x`` as [rows, columns] with unit column stride and rows that do not overlap."""
-    if x.is_cuda and x.dtype in K.DTYPES and x.dim() == 2:      # (mostly all is well)
-        (m, k), (s0, s1) = x.shape, x.stride()
-        if s1 == 1 and k > 0 and (s0 >= k or m <= 1):
-            return x
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be CUDA (sm_100); there is no CPU path")
     if x.dtype not in K.DTYPES:
@@ -93,17 +103,16 @@ def _quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, consta
 
 def quantize_tokens(x: torch.Tensor) -> TokenCodes:
     """int8 codes and a scale for every row of ``x`` [..., in_features] (fp16, bf16 or fp32), in one launch."""
-    x = _rows(x, "x")
-    (m, k), dev = x.shape, x.device
+    x, m, k, stride, dev, code = _matrix(x, "x")
     pitch = (k + 15) & ~15
     codes = _empty(m, pitch, dtype=_int8, device=dev)
     scales = _empty(m, dtype=_float32, device=dev)
     if m:
         # (_quantize, without the calls)
-        desc = _pack_rows(x.data_ptr(), 0, 0, 0, 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0, current_stream_ptr(dev), 0.0, x.stride()[0],
-                          0, 0, 0, pitch, m, k, K.DTYPES[x.dtype], 0, 0, 0)
+        desc = _pack_rows(x.data_ptr(), 0, 0, 0, 0, 0, codes.data_ptr(), scales.data_ptr(), 0, 0, current_stream_ptr(dev), 0.0, stride,
+                          0, 0, 0, pitch, m, k, code, 0, 0, 0)
         K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
-    return TokenCodes(codes if pitch == k else codes[:, :k], scales, None, x.dtype)
+    return TokenCodes(codes if pitch == k else codes[:, :k], scales, None, _TYPES[code])
 
 
 def quantize_channels(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -149,17 +158,17 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
         raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
     if kind == K.NORM_RMS and bias is not None:
         raise ValueError("RMSNorm has no bias")
-    x2 = _rows(x, "x")
-    (m, k), dev = x2.shape, x2.device
-    check_norm(x2, weight, bias, eps)
+    x2, m, k, stride, dev, code = _matrix(x, "x")
+    dtype = _TYPES[code]
+    check_norm(k, dtype, dev, weight, bias, eps)
     res_at = res_stride = hid_at = 0
     hidden = x
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+        res, _, _, res_stride, res_dev, res_code = _matrix(residual, "residual")
+        if residual.shape != x.shape or res_code != code or res_dev != dev:
             raise RuntimeError("residual must have x's shape, type and device")
-        res = _rows(residual, "residual")
-        hidden = _empty(m, k, dtype=x.dtype, device=dev)
-        res_at, res_stride, hid_at = res.data_ptr(), res.stride()[0], hidden.data_ptr()
+        hidden = _empty(m, k, dtype=dtype, device=dev)
+        res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     codes = _new_codes(m, k, dev)
     scales = _empty(m, dtype=_float32, device=dev)
     if m:
@@ -169,17 +178,15 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
             bias = bias.contiguous()
             b_at = bias.data_ptr()
         desc = _pack_rows(x2.data_ptr(), res_at, weight.data_ptr(), b_at, hid_at, 0, codes.data_ptr(), scales.data_ptr(), 0, 0,
-                          current_stream_ptr(dev), eps, x2.stride()[0], res_stride, k, 0, codes.stride()[0], m, k, K.DTYPES[x2.dtype], kind,
-                          0, 0)
+                          current_stream_ptr(dev), eps, stride, res_stride, k, 0, (k + 15) & ~15, m, k, code, kind, 0, 0)
         K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
     if residual is not None and x.dim() != 2:
         hidden = hidden.reshape(x.shape)
-    return TokenCodes(codes, scales, None, x.dtype), hidden
+    return TokenCodes(codes, scales, None, dtype), hidden
 
 
-def check_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
-    """(``x``: what ``_rows`` gave)"""
-    shape, dtype, dev = (x.shape[1],), x.dtype, x.device
+def check_norm(k: int, dtype: torch.dtype, dev: torch.device, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:
+    shape = (k,)
     if weight is None or weight.shape != shape or weight.dtype != dtype or weight.device != dev:
         raise RuntimeError(f"weight must be [{shape[0]}] of x's type on x's device")
     if bias is not None and (bias.shape != shape or bias.dtype != dtype or bias.device != dev):
@@ -242,14 +249,13 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         if out_dtype is None:
             out_dtype = made_of or _float16
     else:
-        x2 = _rows(x, "x")
-        (m, k), dev = x2.shape, x2.device
-        if x.dim() != 2:
+        x2, m, k, x_stride, dev, x_code = _matrix(x, "x")
+        if x2 is not x and x.dim() != 2:
             lead = x.shape[:-1]
         if (L is None) != (R is None):
             raise RuntimeError("a correction needs L and R")
         if out_dtype is None:
-            out_dtype = x2.dtype
+            out_dtype = _TYPES[x_code]
     out_code = K.DTYPES.get(out_dtype)
     if out_code is None:
         raise RuntimeError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
@@ -276,7 +282,7 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         if bias is not None:
             bias = bias.contiguous()
             b_at = bias.data_ptr()
-        rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = x_at = x_stride = x_code = 0
+        rank = mode = L_at = L_stride = R_at = R_stride = r_at = r_stride = rx_at = rx_stride = x_at = 0
         if L is not None:
             rank = L.shape[1] if L.dim() == 2 else 0
             L, L_at, L_stride, copied = _factor(L, "L", oc, None, dev)
@@ -291,15 +297,16 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
             else:
                 R, R_at, R_stride, copied = _factor(R, "R", rank, k, dev)
                 fresh |= copied
-                rx, rx_at, rx_stride, _ = _place((x2 if x2.dtype == _float16 else x2.to(_float16)).detach(), 2)
+                rx, rx_at, rx_stride, _ = _place((x2 if x_code == K.F16 else x2.to(_float16)).detach(), 2)
                 mode = K.R_COMPUTE
         if x2 is None:
             codes, code_at, code_stride, _ = _place(codes, 1)
+            x_stride = x_code = 0
             scales = scales.contiguous()
             scale_at = scales.data_ptr()
         else:
             # codes, scales and r of this call: one piece of memory
-            x_at, x_stride, x_code = x2.data_ptr(), x2.stride()[0], K.DTYPES[x2.dtype]
+            x_at = x2.data_ptr()
             code_stride, r_stride = (k + 15) & ~15, (rank + 7) & ~7
             scale_off = m * code_stride
             r_off = scale_off + (4 * m + 15 & ~15)

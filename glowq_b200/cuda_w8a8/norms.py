@@ -12,23 +12,27 @@ import torch.nn as nn
 
 from ..cuda_w4a16.kernels import current_stream_ptr
 from . import kernels as K
-from .functional import _empty, _float32, _pack_rows, _rows, check_norm
+from .functional import _TYPES, _empty, _float32, _matrix, _pack_rows, _rows, check_norm
 
 
-def _forward(x2, res, weight, bias, eps, statistics: bool):
-    (m, k), dev, dtype = x2.shape, x2.device, x2.dtype
+def _forward(matrix, residual, weight, bias, eps, statistics: bool):
+    """(``matrix``: what ``_matrix`` gave)"""
+    x2, m, k, stride, dev, code = matrix
+    dtype = _TYPES[code]
     y = _empty(m, k, dtype=dtype, device=dev)
     hidden = mean = rstd = None
     res_at = res_stride = hid_at = mean_at = rstd_at = 0
-    if res is not None:
+    if residual is not None:
+        res, _, _, res_stride, _, _ = _matrix(residual, "residual")
         hidden = _empty(m, k, dtype=dtype, device=dev)
-        res_at, res_stride, hid_at = res.data_ptr(), res.stride()[0], hidden.data_ptr()
+        res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     if statistics:
         mean, rstd = _empty(m, dtype=_float32, device=dev), _empty(m, dtype=_float32, device=dev)
         mean_at, rstd_at = mean.data_ptr(), rstd.data_ptr()
     if m:
+        weight, bias = weight.contiguous(), bias.contiguous() if bias is not None else None
         desc = _pack_rows(x2.data_ptr(), res_at, weight.data_ptr(), bias.data_ptr() if bias is not None else 0, hid_at, y.data_ptr(), 0, 0,
-                          mean_at, rstd_at, current_stream_ptr(dev), eps, x2.stride()[0], res_stride, k, k, 0, m, k, K.DTYPES[dtype],
+                          mean_at, rstd_at, current_stream_ptr(dev), eps, stride, res_stride, k, k, 0, m, k, code,
                           K.NORM_LAYER, 0, 0)
         K.call(K.ext().layer_norm_forward, dev, desc, "glowq_layer_norm_forward")
     return y, hidden, mean, rstd
@@ -55,10 +59,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps):
         ctx.set_materialize_grads(False)
-        x2 = _rows(x, "x")
-        res = _rows(residual, "residual") if residual is not None else None
-        w, b = weight.contiguous(), bias.contiguous() if bias is not None else None
-        y, hidden, mean, rstd = _forward(x2, res, w, b, eps, True)
+        y, hidden, mean, rstd = _forward(_matrix(x, "x"), residual, weight, bias, eps, True)
         if residual is None:
             ctx.save_for_backward(x, weight, mean, rstd)
             return y.reshape(x.shape)
@@ -90,16 +91,17 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Layer norm over the last dimension (fp16, bf16 or fp32; ``weight`` and ``bias`` [columns] of the same type): y, or with ``residual``
     (y, h) for h = x + residual.  Differentiable once in all tensors; the gradient of h as an output joins that of y."""
-    x2 = _rows(x, "x")
-    check_norm(x2, weight, bias, eps)
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    matrix = _matrix(x, "x")
+    _, _, k, _, dev, code = matrix
+    dtype = _TYPES[code]
+    check_norm(k, dtype, dev, weight, bias, eps)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != dtype or residual.device != dev):
         raise RuntimeError("residual must have x's shape, type and device")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, residual, float(eps))
-    res = _rows(residual, "residual") if residual is not None else None
-    y, hidden, _, _ = _forward(x2, res, weight.contiguous(), bias.contiguous() if bias is not None else None, eps, False)
-    if x.dim() != 2:
+    y, hidden, _, _ = _forward(matrix, residual, weight, bias, eps, False)
+    if matrix[0] is not x and x.dim() != 2:
         y = y.reshape(x.shape)
         hidden = hidden.reshape(x.shape) if hidden is not None else None
     return y if residual is None else (y, hidden)
