@@ -9,6 +9,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from ..cuda_w4a16.kernels import current_stream_ptr
 from . import kernels as K
@@ -90,15 +91,18 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Layer norm over the last dimension (fp16, bf16 or fp32; ``weight`` and ``bias`` [columns] of the same type): y, or with ``residual``
-    (y, h) for h = x + residual.  Differentiable once in all tensors; the gradient of h as an output joins that of y."""
+    (y, h) for h = x + residual.  Differentiable once in all tensors; the gradient of h as an output joins that of y.  There are no
+    forward-mode derivatives: a dual tensor raises."""
     matrix = _matrix(x, "x")
     _, _, k, _, dev, code = matrix
     dtype = _TYPES[code]
     check_norm(k, dtype, dev, weight, bias, eps)
     if residual is not None and (residual.shape != x.shape or residual.dtype != dtype or residual.device != dev):
         raise RuntimeError("residual must have x's shape, type and device")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    # (under a level of forward-mode derivatives autograd looks at the tensors, and refuses those with a tangent)
+    if forward_ad._current_level >= 0 or (
+            torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                         or (residual is not None and residual.requires_grad))):
         return _LayerNorm.apply(x, weight, bias, residual, float(eps))
     y, hidden, _, _ = _forward(matrix, residual, weight, bias, eps, False)
     if matrix[0] is not x and x.dim() != 2:
