@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from ..cuda_w4a16.kernels import current_stream_ptr
 from . import kernels as K
@@ -152,7 +153,8 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
 
     ``norm``: "layer" (``nn.LayerNorm``'s arithmetic, ``bias`` may be None) or "rms" (the models' RMSNorm modules: fp32 statistics, the
     normalised value rounded to the input's type before the weight).  All tensors have one type; h and the normalised values are
-    rounded to it, so the codes are those of the separate steps."""
+    rounded to it, so the codes are those of the separate steps.  h has the gradients of the sum that it is (and no forward-mode
+    derivatives: a dual tensor raises); the codes have none, as the linears that take them."""
     kind = _NORMS.get(norm)
     if kind is None:
         raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
@@ -161,13 +163,38 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     x2, m, k, stride, dev, code = _matrix(x, "x")
     dtype = _TYPES[code]
     check_norm(k, dtype, dev, weight, bias, eps)
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != dtype or residual.device != dev:
+            raise RuntimeError("residual must have x's shape, type and device")
+        if forward_ad._current_level >= 0 or ((x.requires_grad or residual.requires_grad) and torch.is_grad_enabled()):
+            hidden, codes, scales = _NormCodes.apply(x, residual, weight, bias, eps, kind)
+            return TokenCodes(codes, scales, None, dtype), hidden
+    codes, scales, hidden = _norm_codes(x, (x2, m, k, stride, dev, code), weight, bias, eps, residual, kind)
+    return TokenCodes(codes, scales, None, dtype), hidden
+
+
+class _NormCodes(torch.autograd.Function):
+    """The sum of a call with a residual, with its gradients."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, kind):
+        codes, scales, hidden = _norm_codes(x, _matrix(x, "x"), weight, bias, eps, residual, kind)
+        ctx.mark_non_differentiable(codes, scales)
+        return hidden, codes, scales
+
+    @staticmethod
+    def backward(ctx, dh, *_):
+        return dh, dh, None, None, None, None
+
+
+def _norm_codes(x, matrix, weight, bias, eps, residual, kind):
+    x2, m, k, stride, dev, code = matrix
     res_at = res_stride = hid_at = 0
     hidden = x
     if residual is not None:
-        res, _, _, res_stride, res_dev, res_code = _matrix(residual, "residual")
-        if residual.shape != x.shape or res_code != code or res_dev != dev:
-            raise RuntimeError("residual must have x's shape, type and device")
-        hidden = _empty(m, k, dtype=dtype, device=dev)
+        res, _, _, res_stride, _, _ = _matrix(residual, "residual")
+        # (of x's shape from the start: autograd takes no change in place of a view that a function returns)
+        hidden = _empty(m, k, dtype=_TYPES[code], device=dev) if x2 is x else _empty(x.shape, dtype=_TYPES[code], device=dev)
         res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     codes = _new_codes(m, k, dev)
     scales = _empty(m, dtype=_float32, device=dev)
@@ -180,9 +207,7 @@ def norm_quantize_tokens(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
         desc = _pack_rows(x2.data_ptr(), res_at, weight.data_ptr(), b_at, hid_at, 0, codes.data_ptr(), scales.data_ptr(), 0, 0,
                           current_stream_ptr(dev), eps, stride, res_stride, k, 0, (k + 15) & ~15, m, k, code, kind, 0, 0)
         K.call(K.ext().quantize, dev, desc, "glowq_w8a8_quantize")
-    if residual is not None and x.dim() != 2:
-        hidden = hidden.reshape(x.shape)
-    return TokenCodes(codes, scales, None, dtype), hidden
+    return codes, scales, hidden
 
 
 def check_norm(k: int, dtype: torch.dtype, dev: torch.device, weight: torch.Tensor, bias: Optional[torch.Tensor], eps: float) -> None:

@@ -25,3 +25,36 @@ def test_dual_tensors_are_refused():
                 y, h = norm(x, t)
                 assert torch.equal(h, x + t)
     assert torch.isfinite(norm(x)).all()
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("shape", [(5, 64), (2, 3, 37), (48,)])
+def test_the_sum_in_front_of_codes_has_gradients(shape, norm):
+    a, b, d = (torch.randn(shape, device="cuda") for _ in range(3))
+    w = torch.ones(shape[-1], device="cuda", requires_grad=True)
+    with torch.no_grad():
+        codes, h0 = norm_quantize_tokens(a, w, residual=b, norm=norm)
+    assert not h0.requires_grad and h0.shape == shape
+    for ga, gb in ((True, True), (True, False), (False, True), (False, False)):
+        x, res = a.clone().requires_grad_(ga), b.clone().requires_grad_(gb)
+        t, h = norm_quantize_tokens(x, w, residual=res, norm=norm)
+        assert torch.equal(h, a + b) and torch.equal(t.codes, codes.codes) and torch.equal(t.scales, codes.scales)
+        assert h.shape == shape and h.requires_grad == (ga or gb) and not t.codes.requires_grad and not t.scales.requires_grad
+        assert t.codes.shape == codes.codes.shape and t.codes.stride() == codes.codes.stride()
+        if ga or gb:
+            (h * 2).backward(d)
+        for leaf, g in ((x, ga), (res, gb)):
+            assert (leaf.grad is not None) == g
+            if g:
+                assert torch.equal(leaf.grad, 2 * d)
+    x = a.clone().requires_grad_()
+    t, h = norm_quantize_tokens(x, w, residual=x, norm=norm)      # the same tensor twice
+    h = h.mul_(3.0)                                               # (what is changed in place goes on as any tensor)
+    h.backward(d)
+    assert torch.equal(x.grad, 6 * d)
+    t, h = norm_quantize_tokens(x, w, norm=norm)
+    assert h is x
+    with torch.no_grad(), fw.dual_level():
+        with pytest.raises(NotImplementedError):
+            norm_quantize_tokens(fw.make_dual(a, b), w, residual=b, norm=norm)
+        assert torch.equal(norm_quantize_tokens(a, w, residual=b, norm=norm)[1], a + b)
