@@ -16,16 +16,17 @@ from . import kernels as K
 from .functional import _TYPES, _empty, _float32, _matrix, _pack_rows, _rows, check_norm
 
 
-def _forward(matrix, residual, weight, bias, eps, statistics: bool):
-    """(``matrix``: what ``_matrix`` gave)"""
+def _forward(x, matrix, residual, weight, bias, eps, statistics: bool):
+    """(``matrix``: what ``_matrix`` gave of x.)  Outputs have x's shape from the start: autograd takes no change in place of a view that a
+    function returns."""
     x2, m, k, stride, dev, code = matrix
-    dtype = _TYPES[code]
-    y = _empty(m, k, dtype=dtype, device=dev)
+    dtype, shape = _TYPES[code], (m, k) if x2 is x else x.shape
+    y = _empty(shape, dtype=dtype, device=dev)
     hidden = mean = rstd = None
     res_at = res_stride = hid_at = mean_at = rstd_at = 0
     if residual is not None:
         res, _, _, res_stride, _, _ = _matrix(residual, "residual")
-        hidden = _empty(m, k, dtype=dtype, device=dev)
+        hidden = _empty(shape, dtype=dtype, device=dev)
         res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     if statistics:
         mean, rstd = _empty(m, dtype=_float32, device=dev), _empty(m, dtype=_float32, device=dev)
@@ -60,13 +61,12 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps):
         ctx.set_materialize_grads(False)
-        y, hidden, mean, rstd = _forward(_matrix(x, "x"), residual, weight, bias, eps, True)
+        y, hidden, mean, rstd = _forward(x, _matrix(x, "x"), residual, weight, bias, eps, True)
         if residual is None:
             ctx.save_for_backward(x, weight, mean, rstd)
-            return y.reshape(x.shape)
-        hidden = hidden.reshape(x.shape)
+            return y
         ctx.save_for_backward(hidden, weight, mean, rstd)
-        return y.reshape(x.shape), hidden
+        return y, hidden
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -104,10 +104,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                          or (residual is not None and residual.requires_grad))):
         return _LayerNorm.apply(x, weight, bias, residual, float(eps))
-    y, hidden, _, _ = _forward(matrix, residual, weight, bias, eps, False)
-    if matrix[0] is not x and x.dim() != 2:
-        y = y.reshape(x.shape)
-        hidden = hidden.reshape(x.shape) if hidden is not None else None
+    y, hidden, _, _ = _forward(x, matrix, residual, weight, bias, eps, False)
     return y if residual is None else (y, hidden)
 
 

@@ -58,3 +58,23 @@ def test_the_sum_in_front_of_codes_has_gradients(shape, norm):
         with pytest.raises(NotImplementedError):
             norm_quantize_tokens(fw.make_dual(a, b), w, residual=b, norm=norm)
         assert torch.equal(norm_quantize_tokens(a, w, residual=b, norm=norm)[1], a + b)
+
+
+@pytest.mark.parametrize("shape", [(48,), (6, 48), (2, 3, 48), (2, 1, 3, 37)])
+def test_outputs_that_are_changed_in_place(shape):
+    x, res, d, e = (torch.randn(shape, device="cuda") for _ in range(4))
+    w, b = torch.randn(shape[-1], device="cuda", requires_grad=True), torch.randn(shape[-1], device="cuda", requires_grad=True)
+    leaf, other = x.clone().requires_grad_(), x.clone().requires_grad_()
+    layer_norm(leaf, w, b).mul_(2.0).add_(1.0).backward(d)
+    want = torch.autograd.grad(layer_norm(other, w, b) * 2.0, other, d)[0]
+    assert torch.equal(leaf.grad, want)
+    leaf, other = x.clone().requires_grad_(), x.clone().requires_grad_()
+    y, _ = layer_norm(leaf, w, b, 1e-5, res)
+    y.mul_(2.0).backward(d)
+    y, _ = layer_norm(other, w, b, 1e-5, res)
+    (y * 2.0).backward(d)
+    assert y.shape == shape and torch.equal(leaf.grad, other.grad)
+    y, h = layer_norm(leaf, w, b, 1e-5, res)
+    h.add_(1.0)                               # h is what the gradients are taken from
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.backward((y, h), (d, e))
