@@ -109,7 +109,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
 
 class CudaLayerNorm(nn.LayerNorm):
-    """``nn.LayerNorm`` over the last dimension on the kernels of this package.  ``forward(x, residual)`` returns (y, x + residual)."""
+    """``nn.LayerNorm`` over the last dimension on the kernels of this package.  ``forward(x, residual)`` returns (y, x + residual).
+
+    Under autocast rows and parameters may be of different types, and y is then fp32 as ``nn.LayerNorm``'s there; outside of it they are
+    refused, as ``nn.LayerNorm`` refuses them on this device."""
 
     def __init__(self, normalized_shape, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None, dtype=None):
         super().__init__(normalized_shape, eps, elementwise_affine, bias, device, dtype)
@@ -117,7 +120,13 @@ class CudaLayerNorm(nn.LayerNorm):
             raise ValueError("CudaLayerNorm normalises the last dimension and has a weight")
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
-        return layer_norm(x, self.weight, self.bias, self.eps, residual)
+        weight, bias = self.weight, self.bias
+        if x.dtype != weight.dtype and torch.is_autocast_enabled("cuda"):
+            if residual is not None:
+                h = x + residual
+                return self.forward(h), h
+            x, weight, bias = x.float(), weight.float(), bias.float() if bias is not None else None
+        return layer_norm(x, weight, bias, self.eps, residual)
 
     @classmethod
     def from_float(cls, norm: nn.LayerNorm) -> "CudaLayerNorm":
