@@ -280,7 +280,8 @@ class AddSVDCorrection(nn.Module):
     """``inner(x) + alpha_svd * (x B_q^T) A_q^T`` (src/step3_eval_dataset.py:450-516), fused into one launch.
 
     ``inner`` may be a ``CudaW8A8Linear`` as well: a call then makes the codes of x, r = x B_q^T and the product of its own, and takes nothing
-    from an earlier one.  Members of a group share that work where the caller says so: ``tokens(x)`` of one of them gives ``TokenCodes``
+    from an earlier one.  ``A_q B_q`` then stands for what 8 bits have left of the weight, ``W - inner.dequantized_weight()``; the factors of
+    a 4-bit module stand for its own, larger error and would be added on top.  Members of a group share that work where the caller says so: ``tokens(x)`` of one of them gives ``TokenCodes``
     that all take in the place of x."""
 
     def __init__(self, inner: nn.Module, A_q: torch.Tensor, B_q: torch.Tensor, role: str, is_group: bool,
@@ -415,9 +416,20 @@ def _resolve(bkey: str, module_name: str):
     return gkey, gkey + ".A", "solo", False
 
 
+def _too_large(inner: CudaW8A8Linear, w: AddSVDCorrection) -> bool:
+    """Whether a correction is larger than all that rounding to 8 bits has left of the weight: a step of scale_o leaves an error of
+    scale_o^2 / 12 in the mean square, and a part of that error is no larger than the whole."""
+    if w._mismatch or w.A_q.device.type == "meta":
+        return False
+    A, B = w.A_q.double(), w.B_q.double()
+    square = ((A.t() @ A) * (B @ B.t())).sum() * float(w.alpha_svd) ** 2          # |alpha A B|^2
+    left = inner.scales_f32.double().square().sum() * inner.in_features / 12
+    return bool(square > left)
+
+
 def _patch(model, shared, bmap, alpha_svd, groups_to_patch: Optional[Set[str]], verbose: bool):
     patched = skipped = 0
-    wrapped = []
+    wrapped, large = [], []
     caches: Dict[str, MiniGroupCache] = {}
     items = bmap.items()
     if verbose:
@@ -449,9 +461,15 @@ def _patch(model, shared, bmap, alpha_svd, groups_to_patch: Optional[Set[str]], 
         setattr(parent, leaf, wrapper)
         if isinstance(inner, CudaW4A16Linear):      # (launchers join the members of 4-bit groups)
             wrapped.append((gkey, wrapper))
+        elif _too_large(inner, wrapper):
+            large.append(module_name)
         patched += 1
     if verbose:
         print(f"SVD Correction Patching Summary: {patched} patched, {skipped} skipped")
+    if large:
+        warnings.warn(f"{len(large)} 8-bit modules (the first: {large[0]}) were given corrections that are larger than all that 8 bits have left "
+                      "of their weights, as factors of the 4-bit error are: they make the results worse. Factors of an 8-bit module are "
+                      "fitted to W - module.dequantized_weight()")
     if _fuse_enabled():
         # launch order = module order of the model (q, k, v, o, gate, up, down within a layer), whatever the order of
         # the map's entries

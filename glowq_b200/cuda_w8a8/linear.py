@@ -39,6 +39,11 @@ class CudaW8A8Linear(nn.Module):
         w = self.qweight_i8
         return w if w.shape[1] == self.in_features else w[:, :self.in_features]
 
+    def dequantized_weight(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The weight that the codes stand for, [out_features, in_features]: what is left of the original, ``W - dequantized_weight()``, is what
+        a correction's factors are fitted to."""
+        return (self.weight_codes.float() * self.scales_f32[:, None]).to(dtype)
+
     def launch(self, x: Union[torch.Tensor, TokenCodes], *, L=None, R=None, alpha: float = 1.0) -> torch.Tensor:
         """The linear, optionally with its low-rank correction folded in."""
         return w8a8_linear(x, self.weight_codes, self.scales_f32, self.bias, out_dtype=self.out_dtype, L=L, R=R, alpha=alpha)
