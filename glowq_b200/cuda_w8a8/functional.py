@@ -54,8 +54,12 @@ def _matrix(x: torch.Tensor, name: str):
         shape = x.shape
         if len(shape) == 2:
             (m, k), (s0, s1) = shape, x.stride()
+            if m.__class__ is not int:      # (sizes are tensors under a trace)
+                K.refuse_trace()
             if s1 == 1 and k > 0 and (s0 >= k or m <= 1):
                 return x, m, k, s0, x.device, code
+    if K.tracing():
+        K.refuse_trace()
     x = _rows(x, name)
     return x, x.shape[0], x.shape[1], x.stride()[0], x.device, K.DTYPES[x.dtype]
 
@@ -77,11 +81,11 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     return x
 
 
-def _place(t: torch.Tensor, e: int):
-    """(tensor, address, row stride, flag) of a matrix of ``e``-byte elements as the copy engine reads it: rows that begin on 16 bytes.
+def _place(t: torch.Tensor, e: int, rows: int, cols: int):
+    """(tensor, address, row stride, flag) of a matrix [rows, cols] of ``e``-byte elements as the copy engine reads it: rows that begin on 16 bytes.
     (Others are copied; what the package makes lies so.  Of a single row the stride may be anything: the library is told one that it
     accepts.)  The flag is ``K.FRESH`` for a copy, which a launch right behind it may not read early, else 0."""
-    at, (rows, cols), (s0, s1) = t.data_ptr(), t.shape, t.stride()
+    at, (s0, s1) = t.data_ptr(), t.stride()
     if not at & 15 and s1 == 1:
         if rows > 1:
             if s0 >= cols and not s0 * e & 15:
@@ -135,8 +139,7 @@ def channel_rows(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if oc == 0:
         return rows, scales
     if weight.is_cuda:
-        weight = _rows(weight, "weight")
-        _quantize(weight, codes, scales, True)
+        _quantize(_matrix(weight, "weight")[0], codes, scales, True)
         return rows, scales
     top = weight.float().abs().amax(dim=1)
     torch.div(top, torch.full_like(top, 127.0), out=scales)
@@ -194,7 +197,7 @@ def _norm_codes(x, matrix, weight, bias, eps, residual, kind):
     if residual is not None:
         res, _, _, res_stride, _, _ = _matrix(residual, "residual")
         # (of x's shape from the start: autograd takes no change in place of a view that a function returns)
-        hidden = _empty(m, k, dtype=_TYPES[code], device=dev) if x2 is x else _empty(x.shape, dtype=_TYPES[code], device=dev)
+        hidden = _empty(m, k, dtype=_TYPES[code], device=dev) if x2 is x else _empty(*x.shape, dtype=_TYPES[code], device=dev)
         res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     codes = _new_codes(m, k, dev)
     scales = _empty(m, dtype=_float32, device=dev)
@@ -222,18 +225,18 @@ def check_norm(k: int, dtype: torch.dtype, dev: torch.device, weight: torch.Tens
 
 def _factor(t: torch.Tensor, name: str, rows: int, cols: Optional[int], device):
     """(``_place`` of a factor)"""
-    if t.dtype != _float16 or t.device != device or t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
-        raise RuntimeError(f"{name} must be fp16 [{rows}, {'rank' if cols is None else cols}] on {device}, got {t.dtype} {tuple(t.shape)}")
-    return _place(t.detach() if t.requires_grad else t, 2)
+    shape = t.shape
+    if t.dtype != _float16 or t.device != device or len(shape) != 2 or shape[0] != rows or (cols is not None and shape[1] != cols):
+        raise RuntimeError(f"{name} must be fp16 [{rows}, {'rank' if cols is None else cols}] on {device}, got {t.dtype} {tuple(shape)}")
+    return _place(t.detach() if t.requires_grad else t, 2, rows, shape[1])
 
 
 def right_factor(x: torch.Tensor, R: torch.Tensor, constant: bool = True) -> torch.Tensor:
     """r = x R^T, fp16 [tokens, rank], for corrected linears that share a right factor (``TokenCodes.r``).  ``x`` is taken in fp16, as the
     W4A16 path takes it; sums in fp32.  ``constant``: as for ``w8a8_linear``."""
-    x = _rows(x.detach(), "x")
+    x, m, k, _, dev, code = _matrix(x.detach(), "x")
     if R.dim() != 2 or not 0 < R.shape[0] <= K.MAX_RANK:
         raise RuntimeError(f"R must be [rank, in_features] with a rank of 1 to {K.MAX_RANK}")
-    (m, k), dev = x.shape, x.device
     if m > K.MAX_TOKENS:
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
     R, R_at, R_stride, fresh = _factor(R, "R", R.shape[0], k, dev)
@@ -243,7 +246,7 @@ def right_factor(x: torch.Tensor, R: torch.Tensor, constant: bool = True) -> tor
     pitch = (rank + 7) & ~7
     r = _empty(m, pitch, dtype=_float16, device=dev)
     if m:
-        x, x_at, x_stride, _ = _place(x if x.dtype == _float16 else x.to(_float16), 2)
+        x, x_at, x_stride, _ = _place(x if code == K.F16 else x.to(_float16), 2, m, k)
         desc = _pack_linear(0, 0, 0, 0, 0, 0, x_at, R_at, r.data_ptr(), 0, 0, current_stream_ptr(dev), 0, 0, 0, x_stride, R_stride, pitch, 0,
                             0, m, k, 0, rank, 0, 0, K.R_COMPUTE | fresh, 0.0, 0)
         K.call(K.ext().right_factor, dev, desc, "glowq_w8a8_right_factor")
@@ -264,9 +267,12 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     x2 = lead = r = None
     if isinstance(x, TokenCodes):
         codes, scales, r, made_of = x
-        if not codes.is_cuda or codes.dtype != _int8 or codes.dim() != 2:
+        shape, dev = codes.shape, codes.device
+        if not codes.is_cuda or codes.dtype != _int8 or len(shape) != 2:
             raise RuntimeError("codes must be int8 [tokens, in_features] on a CUDA device")
-        (m, k), dev = codes.shape, codes.device
+        m, k = shape
+        if m.__class__ is not int:
+            K.refuse_trace()
         if scales.dtype != _float32 or scales.shape != (m,) or scales.device != dev:
             raise RuntimeError(f"scales must be fp32 [{m}] on {dev}")
         if R is not None:
@@ -284,9 +290,10 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     out_code = K.DTYPES.get(out_dtype)
     if out_code is None:
         raise RuntimeError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
-    if weight.dtype != _int8 or weight.dim() != 2 or weight.device != dev:
+    shape = weight.shape
+    if weight.dtype != _int8 or len(shape) != 2 or weight.device != dev:
         raise RuntimeError(f"weight must be int8 [out_features, in_features] on {dev}")
-    oc, ic = weight.shape
+    oc, ic = shape
     if ic != k:
         raise ValueError(f"Input dim mismatch: got {k}, expected {ic}")
     if not 0 < k <= K.MAX_EXACT_K:
@@ -299,7 +306,7 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
         raise RuntimeError(f"at most {K.MAX_TOKENS} tokens")
     out = _empty(m, oc, dtype=out_dtype, device=dev)
     if m and oc:
-        weight, w_at, w_stride, fresh = _place(weight, 1)
+        weight, w_at, w_stride, fresh = _place(weight, 1, oc, ic)
         if not constant:
             fresh = K.FRESH
         weight_scales = weight_scales.contiguous()
@@ -322,10 +329,10 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
             else:
                 R, R_at, R_stride, copied = _factor(R, "R", rank, k, dev)
                 fresh |= copied
-                rx, rx_at, rx_stride, _ = _place((x2 if x_code == K.F16 else x2.to(_float16)).detach(), 2)
+                rx, rx_at, rx_stride, _ = _place((x2 if x_code == K.F16 else x2.to(_float16)).detach(), 2, m, k)
                 mode = K.R_COMPUTE
         if x2 is None:
-            codes, code_at, code_stride, _ = _place(codes, 1)
+            codes, code_at, code_stride, _ = _place(codes, 1, m, k)
             x_stride = x_code = 0
             scales = scales.contiguous()
             scale_at = scales.data_ptr()

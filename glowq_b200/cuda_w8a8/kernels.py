@@ -81,8 +81,13 @@ def ext() -> _Ext:
 
 
 _device_now = K.current_device
-_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+tracing = torch.jit.is_tracing
 _modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def refuse_trace():
+    raise RuntimeError("the 8-bit path cannot be traced (torch.jit.trace, make_fx): a trace does not see its launches and would keep nothing "
+                       "but the allocation of their outputs; capture a CUDA graph")
 
 
 def _proxies() -> bool:
@@ -90,10 +95,9 @@ def _proxies() -> bool:
 
 
 def call(fn, device: torch.device, desc: bytes, what: str) -> None:
-    """``fn(desc)`` with ``device`` current.  Not under a trace of torch's operations, which does not see these calls and would keep
-    nothing but the allocation of their outputs."""
-    if _tracing() or (_modes() and _proxies()):
-        raise RuntimeError(f"{what} cannot be traced (torch.jit.trace, make_fx); capture a CUDA graph")
+    """``fn(desc)`` with ``device`` current.  (What a trace by ``torch.jit`` gives as sizes is refused where sizes are read.)"""
+    if _modes() and _proxies():
+        refuse_trace()
     if _device_now() == device.index:
         rc = fn(desc)
     else:

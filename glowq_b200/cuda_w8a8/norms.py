@@ -21,12 +21,12 @@ def _forward(x, matrix, residual, weight, bias, eps, statistics: bool):
     function returns."""
     x2, m, k, stride, dev, code = matrix
     dtype, shape = _TYPES[code], (m, k) if x2 is x else x.shape
-    y = _empty(shape, dtype=dtype, device=dev)
+    y = _empty(*shape, dtype=dtype, device=dev)
     hidden = mean = rstd = None
     res_at = res_stride = hid_at = mean_at = rstd_at = 0
     if residual is not None:
         res, _, _, res_stride, _, _ = _matrix(residual, "residual")
-        hidden = _empty(shape, dtype=dtype, device=dev)
+        hidden = _empty(*shape, dtype=dtype, device=dev)
         res_at, hid_at = res.data_ptr(), hidden.data_ptr()
     if statistics:
         mean, rstd = _empty(m, dtype=_float32, device=dev), _empty(m, dtype=_float32, device=dev)
