@@ -5,16 +5,19 @@
 // All of it is bound by memory: a row is read once, stays in registers through the norm, the maximum and the codes, and every output is
 // written once.  A row belongs to a CTA of as many threads as it has pieces of 4 x 16 bytes (to one warp up to 1024 16-bit columns,
 // several rows to a CTA then).  Values stay in their own type in registers (16 for 32 16-bit values), so that an SM holds 1024 threads'
-// rows; above 256 threads a row, CTAs take row after row, and a row's loads go out before the row in front of it is worked on.
+// rows; above 256 threads a row, CTAs take row after row, and a row's loads go out before the row in front of it is worked on.  64
+// registers do not hold all of that beside the arithmetic: behind a norm the compiler spills 10 to 100 bytes a thread (fp32: none to 100),
+// with the next row in flight and a residual 140 (RMSNorm) to 240 (layer norm), with eight pieces a thread 160 to 420.
 //   Rows that do not begin on 16 bytes are read in 16-byte pieces all the same (see Mode).  (Element by element 4097 x 4999 fp16 took
-// 39 us, floor 9.4; so 16.)
+// 39 us, floor 9.4; so 20.)
 //   A code is the nearest integer of the EXACT quotient, ties to even: it does not hang on how a division rounds.  Products with a little
 // less and a little more than 1 / s have the same nearest integer but where a border is near (one value in some ten thousand; of 8-bit
 // mantissas, many of whose quotients are halves, one in some hundred); there the side of the border that v is on decides, which one FMA
 // gives exactly.
-//   us (floor): codes of 4096 x 13824 fp16 28.2 (26.0), bf16 32.8, fp32 44.3 (43.3); residual + RMSNorm + codes of 4000 x 5120 fp16 25.5
-// (21.9), with a layer norm 28.6; layer norm of 32768 x 2048 fp16 47.6 (41.1).  What is left is bound by issue slots: 11 to 25 instructions
-// an element.
+//   us (floor), normal values: codes of 4096 x 13824 fp16 29.0 (26.0), bf16 33.1 (29.8 of activations with some loud channels, whose
+// quotients are halves less often), fp32 45.0 (43.3); residual + RMSNorm + codes of 4000 x 5120 fp16 25.7 (21.9), with a layer norm 29.3,
+// of 4000 x 12288 81 and 101 (52.6); layer norm of 32768 x 2048 fp16 47.5 (41.1).  What is left is bound by issue slots: 11 to 25
+// instructions an element, and above 8192 columns by the spills.
 //   The statistics of a norm are sums in 64 bits, rounded to fp32 once, so that they - and with them every code - do not depend on the
 // order of the sums.  var = S2/K - (S1/K)^2 from one pass over the registers; where the difference costs more than 20 of the 53 bits (rows
 // whose mean is a thousand times their deviation) a second pass sums the squares around the mean.
@@ -754,8 +757,8 @@ template <typename T, int NORM, bool RES, bool CODES> cudaError_t launch_rows_of
       on16(p.bias) && codes)
     return launch_rows_cut<T, NORM, RES, CODES, kWhole>(p, sms, stream);
   // Codes alone: x is the only matrix whose rows may lie anywhere; shifting what is read takes less than shifting codes (20000 x 2999 fp16
-  // 55 us, so 70).  Behind a norm the rows' own places are taken where all matrices share them (6000 x 9001 bf16 with a residual 109 us,
-  // so 295); matrices that do not take passes over the row.
+  // 54 us, so 70).  Behind a norm the rows' own places are taken where all matrices share them (6000 x 9001 bf16 with a residual and
+  // RMSNorm 148 us, 20000 x 2999 fp16 168); matrices that do not take passes over the row (315 and 413).
   if constexpr (NORM == GLOWQ_NORM_NONE) {
     return launch_rows_cut<T, NORM, RES, CODES, kAny>(p, sms, stream);
   } else {
@@ -781,9 +784,11 @@ template <typename T> cudaError_t launch_rows_typed(const RowsParams& p, int nor
 // ---------------------------------------------------------------- gradients of the layer norm
 // A CTA holds one or several groups of threads that have a row's columns between them (NV pieces of 16 bytes a thread); a group takes ROWS
 // rows at a time, and the next ones' loads go out before these are worked on.  A thread keeps to its columns: the sums of dweight and
-// dbias stay in its registers until the end.  Reads h, dy (dh) and writes dx once.  32768 x 2048 fp16 87 us (floor 61.6), 8192 x 5120 bf16
-// 79 (38.5): bound by issue slots, 23 instructions an element, a third of them moves and addresses, and by a barrier for every round.
-// (A warp along each row first and threads down its columns then, the second reads from L1: 26 instructions, 117 us.)
+// dbias stay in its registers until the end.  Reads h, dy (dh) and writes dx once.  32768 x 2048 fp16 90 us (floor 61.6): bound by issue
+// slots, 24.5 instructions an element, a third of them moves and addresses, and by a barrier for every round.  Wider rows (16 bits: above 2048
+// columns) go one at a time through CTAs of 64 registers a thread: 8192 x 5120 bf16 80 us (38.5) with 35 instructions an element, fp32 130
+// (77); with two pieces a thread, which spill 430 bytes a thread of 16-bit rows, 8192 x 9216 bf16 252 (69), 8192 x 12288 297 (92).
+// (A warp along each row first and threads down its columns then, the second reads from L1: 2048 columns 26 instructions, 117 us.)
 constexpr int kGradParts = 304;    // CTAs of the gradients at most, whatever the device: their number fixes the order of the sums
 constexpr int kGradThreads = 1024;
 
@@ -1040,7 +1045,8 @@ struct GradPlan {
 GradPlan grad_plan(int M, int K, int vec, bool same) {
   GradPlan g{};
   const int n = (K + vec - 1) / vec + (same ? 1 : 0);
-  // (two 16-bit pieces that are shifted need more registers than there are: 6000 x 9001 bf16 525 us, in passes over the rows 263)
+  // (two 16-bit pieces that are shifted need more registers than there are: 6000 x 9001 bf16 278 us, in passes over the rows 264; at 12001
+  // and 16001 columns fp16 the passes take 4 to 6 % more)
   g.nv = n <= kGradThreads ? 1 : n <= 2 * kGradThreads && !(same && vec == 8) ? 2 : 0;
   g.group = g.nv ? ((n + g.nv - 1) / g.nv + 31) / 32 * 32 : 256;
   g.groups = g.group >= 256 ? 1 : 256 / g.group;

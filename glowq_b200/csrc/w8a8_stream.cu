@@ -342,7 +342,8 @@ int plan_split(long long tiles, int steps, int sms, int most) {
   return best;
 }
 
-// (sixteen, of an SM each, where r's rows are long: 77 tokens, 18944 columns, rank 128: 13.0 us in eight, 9.7; 7 tokens, 5120: 5.5, so 6.1)
+// (sixteen, of an SM each, where r's rows are long: 77 tokens, 18944 columns (296 steps), rank 128: 13.0 us in eight, 9.7; 7 tokens, 5120
+// columns (80 steps): 5.5, so 6.1.  Nothing between was measured: 160 is twice the one and half the other.)
 int most_split(bool f16, int steps) { return f16 && steps >= 160 ? kMaxSplit : 8; }
 
 template <int N, bool F16, bool TWO>

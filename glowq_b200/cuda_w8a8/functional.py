@@ -260,7 +260,8 @@ def w8a8_linear(x: Union[torch.Tensor, TokenCodes], weight: torch.Tensor, weight
     ``weight`` int8 [out_features, in_features] and ``weight_scales`` fp32 [out_features] as ``quantize_channels`` gives them, ``bias`` fp32
     [out_features].  ``out_dtype``: fp16, bf16 or fp32; by default the activations' type, that which codes
     were made of (fp16 where ``TokenCodes.dtype`` is None).  ``L`` fp16 [out_features, rank]:
-    the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``.
+    the linear is corrected by alpha * r L^T, with r = x R^T (``R`` fp16 [rank, in_features]) or the codes' ``r``.  r is made of x in fp16 and
+    held in fp16, as the W4A16 path has it: of a bf16 or fp32 token whose values or r pass 65504 the corrected outputs are not finite.
 
     ``constant``: ``weight``, ``L`` and ``R`` may be read before what is in front of this call on the stream is complete.  Pass False where
     the operation right in front made one of them (a merge, a cast, a copy; what ``quantize_channels`` gives may be used at once)."""

@@ -2,7 +2,8 @@
 
     h = x + residual (rounded to the type of x),  y = (h - mean) * rstd * weight + bias
 
-Statistics are taken in 64 bits and held in fp32, sums of gradients in fp32 in an order that the sizes fix; each output is rounded once."""
+Statistics are taken in 64 bits and held in fp32, sums of gradients in fp32 in an order that the sizes (and the
+rows' places within 16 bytes) fix; each output is rounded once."""
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union

@@ -59,7 +59,8 @@ int glowq_layer_norm_forward(const glowq_w8a8_rows_t* rows);
 
 /* Gradients of the layer norm y = LN(h) * weight + bias, where h may itself be an output (residual form):
  *     g = dy * weight,  xh = (h - mean) * rstd,  dx = rstd * (g - mean_k(g) - xh * mean_k(g xh)) + dh
- *     dweight = sum_t dy xh,  dbias = sum_t dy           (fp32 sums in an order that the sizes fix; rounded once)
+ *     dweight = sum_t dy xh,  dbias = sum_t dy           (fp32 sums in an order that the sizes and the rows'
+ *                                                           places within 16 bytes fix; rounded once)
  * dweight and dbias may be NULL together; dx may be NULL.  `workspace`: glowq_layer_norm_workspace_bytes(), any contents. */
 typedef struct glowq_layer_norm_grad {
   const void* h;
@@ -88,7 +89,8 @@ enum { GLOWQ_W8A8_FRESH = 16 };
 /* One linear.  With `x` set the call first quantises x into `codes` and `scales` (which are then scratch of the caller's); with r_mode
  * GLOWQ_R_COMPUTE it computes r = r_x . R^T (rounded to fp16, as the W4A16 path holds it) into `r`; GLOWQ_R_LOAD takes r as it is.
  * Alignment: codes, weight, r_x, R, L and r begin on 16 bytes and their row strides are multiples of 16 bytes (what lies behind
- * column K is never used); out and bias need the alignment of their elements.  K <= 131071 (exact sums); rank <= 1024; at most 2^22
+ * column K is never used).  r and r_x are fp16: where a token's values or its r pass 65504 its corrected outputs are infinite or NaN,
+ * whatever x_dtype.  out and bias need the alignment of their elements.  K <= 131071 (exact sums); rank <= 1024; at most 2^22
  * tokens and 2^29 channels.
  * `weight`, `weight_scales`, `bias`, L and R are constants: they may be read before what is in front of this call on the stream is complete
  * and visible, whoever launched it.  Where the kernel, copy or call right in front made one of them, add GLOWQ_W8A8_FRESH to r_mode
