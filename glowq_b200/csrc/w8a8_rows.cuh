@@ -19,8 +19,10 @@
 // of 4000 x 12288 81 and 101 (52.6); layer norm of 32768 x 2048 fp16 47.5 (41.1).  What is left is bound by issue slots: 11 to 25
 // instructions an element, and above 8192 columns by the spills.
 //   The statistics of a norm are sums in 64 bits, rounded to fp32 once, so that they - and with them every code - do not depend on the
-// order of the sums.  var = S2/K - (S1/K)^2 from one pass over the registers; where the difference costs more than 20 of the 53 bits (rows
-// whose mean is a thousand times their deviation) a second pass sums the squares around the mean.
+// order of the sums.  var = S2/K - (S1/K)^2 from one pass over the registers; where the difference costs more than 10 of the 53 bits (rows
+// whose mean is 32 times their deviation) a second pass sums the squares around the mean.  (Below that the rounding to 24 bits went another
+// way in less than one row of a million; at 64 deviations in one of 400 thousand, at 900 in one of two thousand.  From memory 4000 x 5120 fp16
+// with codes 29 -> 50 us of such rows; from the registers 36, but then others' spills take 4 to 10 % more at 12288 columns.)
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -585,8 +587,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
       sum = row_sum<WARP, NORM == GLOWQ_NORM_LAYER>(sum, s_sum[buf]);
       const double mean = sum.x * p.inv_k;
       double var = sum.y * p.inv_k - mean * mean;
-      if (NORM == GLOWQ_NORM_LAYER && var < 0x1p-20 * mean * mean) {
-        // more than 20 bits went in the difference: once more, around the mean (and from memory, which takes no registers from the others;
+      if (NORM == GLOWQ_NORM_LAYER && var < 0x1p-10 * mean * mean) {
+        // more than 10 bits went in the difference: once more, around the mean (and from memory, which takes no registers from the others;
         // a quotient, which is exact where the mean is: a constant row's deviation is nothing, not 2^-53 of its value)
         const double mu = sum.x / K;
         double2 s = make_double2(0.0, 0.0);

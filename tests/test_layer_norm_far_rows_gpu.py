@@ -102,3 +102,19 @@ def test_deviation_of_constant_rows(k, dtype):
         assert_within(gx, *dx, "dx")
         assert_within(gb, *db, "db")
         assert not gw.any()
+
+
+@pytest.mark.parametrize("ratio", [3, 20, 100, 900])
+def test_statistics_are_rounded_once(ratio):
+    """Rows whose mean is many deviations: rstd, and with it every scale and code, is that of 64-bit sums."""
+    m, k = 200_000, 200
+    gen = torch.Generator(device="cuda").manual_seed(ratio)
+    x = torch.randn(m, k, generator=gen, device="cuda") + ratio * torch.randn(m, 1, generator=gen, device="cuda").sign()
+    w, b = (1 + 0.3 * torch.randn(k, generator=gen, device="cuda")), 0.3 * torch.randn(k, generator=gen, device="cuda")
+    t, _ = w8.norm_quantize_tokens(x, w, b, eps=EPS, norm="layer")
+    _, y, mean, rstd = norm_of(x, None, w, b, EPS, "layer")
+    out = w8.layer_norm(x.requires_grad_(), w, b, EPS)
+    kept, root = out.grad_fn.saved_tensors[2:]
+    assert torch.equal(kept, mean.flatten()) and torch.equal(root, rstd.flatten())
+    codes, scales = codes_of(y)
+    assert torch.equal(t.scales, scales) and torch.equal(t.codes, codes)
