@@ -670,14 +670,16 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_kernel(const __grid_con
   Stats st{0.f, 1.f};
   if (NORM != GLOWQ_NORM_NONE) {
     double2 sum = make_double2(0.0, 0.0);
-    double mean = 0.0;
+    double mean = 0.0, mu = 0.0;   // (as in rows_kernel: the mean to be held, and that which deviations are taken from)
     if (NORM == GLOWQ_NORM_LAYER) {
       for (int k = threadIdx.x; k < K; k += blockDim.x) sum.x += value(k);
-      mean = row_sum<false, true>(sum, s_sum).x / K;
+      const double total = row_sum<false, true>(sum, s_sum).x;
+      mean = total * p.inv_k;
+      mu = total / K;
       __syncthreads();
     }
     for (int k = threadIdx.x; k < K; k += blockDim.x) {
-      const double d = static_cast<double>(value(k)) - mean;
+      const double d = static_cast<double>(value(k)) - mu;
       sum.y = fma(d, d, sum.y);
     }
     st = make_stats<NORM>(mean, row_sum<false, true>(sum, s_sum).y * p.inv_k, p.eps);
